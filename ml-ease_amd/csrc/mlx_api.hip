@@ -499,6 +499,17 @@ int finish_part(mlx_handle h, PartHost &ph)
 }  // namespace
 
 // =================================================================================================
+int mlxi_fail(int code, const char *fmt, ...)
+{
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    try { g_err_nohandle = buf; } catch (...) { g_err_nohandle.clear(); }
+    return code;
+}
+
 extern "C" {
 
 #ifdef MLX_EXPERIMENTAL

@@ -70,3 +70,6 @@ void mlxk_spin(hipStream_t st, long long ticks);
 // RegressionTest scoring: one float prediction per row
 void mlxk_score_rows(hipStream_t st, int l, const int64_t *rp, const int32_t *gi, const double *val, const double *off,
                      const double *z, double base, float *pred);
+
+// The calling thread's message of mlx_last_error(NULL), for entry points that take no handle (mlx_operators.hip); returns code.
+int mlxi_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));

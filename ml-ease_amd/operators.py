@@ -1,0 +1,200 @@
+"""Operators on token ids, logits and pairs of answers, as torch calls on one MI355X (C-ABI: include/mlease_operators.h).
+
+They stand beside the trainer's own: a lookup of rows by id with a scaling, and its gradient by sorted ids (what
+``HipScorer.score_rows`` and the solver's column pass do at width 1), the log-likelihood of a token among many classes with its
+gradient (``HipAdmmEngine.test_loglik_sums`` for two), and the logistic loss with weight and offset on the margins of pairs.
+
+    ops = HipOperators(device=0)
+    x = ops.embedding_lookup(table, ids, scale=math.sqrt(width))
+    ...                                                     # the caller's own layers
+    logp, stats = ops.token_loglik(logits, target)
+    r = ops.preference_loss(logp, ref_logp, seq_ptr, beta=0.1, scale=1.0 / pairs, mask=mask)
+    dlogits = ops.token_loglik_gradient(logits, target, stats, r.grad, out=logits)
+    ...
+    ops.embedding_gradient(dx, ids, n_rows, scale=math.sqrt(width), out=table_grad, accumulate=True)
+
+Gradients are calls of their own, as everywhere in this package: nothing records them. Every call enqueues its work on torch's
+current stream of the device and returns; it allocates its outputs and workspace from torch on that stream, so that it can be
+captured into a graph and made from several threads and streams. Tensors that were written on another stream need the caller's
+event, as for any torch operation. There is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from collections import namedtuple
+
+from .hip_engine import load_library
+
+# every entry point include/mlease_operators.h declares
+OPERATOR_SYMBOLS = [
+    "mlx_embedding_lookup", "mlx_embedding_gradient_workspace", "mlx_embedding_gradient", "mlx_token_loglik_workspace", "mlx_token_loglik",
+    "mlx_token_loglik_gradient", "mlx_preference_loss_workspace", "mlx_preference_loss",
+]
+
+PreferenceResult = namedtuple("PreferenceResult", "loss pair_loss margin ratio grad")
+
+
+def load_operators():
+    """The HIP library with the operators' argument types declared."""
+    L = load_library()
+    if not getattr(L, "_operators_declared", False):
+        vp, i32, i64, f32, sz = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
+        psz = C.POINTER(sz)
+        L.mlx_embedding_lookup.argtypes = [i32, vp, i32, vp, i64, i64, i64, i32, vp, i64, f32, vp, i64]
+        L.mlx_embedding_gradient_workspace.argtypes = [i64, i64, i64, psz]
+        L.mlx_embedding_gradient.argtypes = [i32, vp, i32, vp, i64, i32, vp, i64, f32, i32, i32, vp, i64, i64, i64, vp, sz]
+        L.mlx_token_loglik_workspace.argtypes = [i64, i64, psz]
+        L.mlx_token_loglik.argtypes = [i32, vp, i32, vp, i64, i64, i64, i32, vp, vp, vp, vp, sz]
+        L.mlx_token_loglik_gradient.argtypes = [i32, vp, i32, vp, i64, i64, i64, i32, vp, vp, vp, vp, i64]
+        L.mlx_preference_loss_workspace.argtypes = [i64, i64, psz]
+        L.mlx_preference_loss.argtypes = [i32, vp, vp, vp, i64, vp, i64, f32, f32, f32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz]
+        L._operators_declared = True
+    return L
+
+
+class HipOperators:
+    """The operators on one device. Arguments that a call cannot take raise ValueError (wrong tensors) or RuntimeError (the library's checks)."""
+
+    def __init__(self, device: int = 0):
+        import torch
+
+        self.L = load_operators()
+        if not torch.cuda.is_available():
+            raise RuntimeError("no HIP device visible: the MI355X path has no CPU fallback")
+        if not 0 <= int(device) < torch.cuda.device_count():
+            raise RuntimeError("device %d out of range (%d devices)" % (device, torch.cuda.device_count()))
+        self.device = int(device)
+        self._setup(torch)
+
+    def _setup(self, torch):
+        self._torch = torch
+        self._at = torch.device("cuda", self.device)
+        self._types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+        self._id_types = {torch.int32: 0, torch.int64: 1}
+
+    # -- checks -----------------------------------------------------------------------------------
+    def _matrix(self, t, what):
+        """(pointer, ld) of a 2-D tensor of this device whose rows are contiguous."""
+        if t.dim() != 2 or t.dtype not in self._types:
+            raise ValueError("%s must be a matrix of float32, bfloat16 or float16, not %d-dimensional %s" % (what, t.dim(), t.dtype))
+        if t.device != self._at:
+            raise ValueError("%s is on %s, these operators are on %s" % (what, t.device, self._at))
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError("the rows of %s must be contiguous (strides %s)" % (what, tuple(t.stride())))
+        return t.data_ptr(), t.stride(0)
+
+    def _vector(self, t, what, n, dtype):
+        if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype:
+            raise ValueError("%s must be a vector of %d %s, not %s %s" % (what, n, dtype, tuple(t.shape), t.dtype))
+        if t.device != self._at:
+            raise ValueError("%s is on %s, these operators are on %s" % (what, t.device, self._at))
+        if n > 1 and t.stride(0) != 1:
+            raise ValueError("%s must be contiguous" % what)
+        return t.data_ptr()
+
+    def _ids(self, t, what, n=None):
+        if t.dim() != 1 or t.dtype not in self._id_types or (n is not None and t.shape[0] != n):
+            raise ValueError("%s must be a vector of %sint32 or int64, not %s %s" % (what, "" if n is None else "%d " % n, tuple(t.shape), t.dtype))
+        return self._vector(t, what, t.shape[0], t.dtype), self._id_types[t.dtype]
+
+    def _output(self, out, what, shape, dtype):
+        if out is None:
+            return self._torch.empty(shape, dtype=dtype, device=self._at)
+        if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+            raise ValueError("%s must be %s %s, not %s %s" % (what, tuple(shape), dtype, tuple(out.shape), out.dtype))
+        return out
+
+    def _workspace(self, query, *sizes):
+        need = C.c_size_t()
+        self._ck(query(*sizes, C.byref(need)))
+        if not need.value:
+            return None, None, 0
+        w = self._torch.empty(need.value, dtype=self._torch.uint8, device=self._at)      # torch's blocks are aligned to 512 bytes
+        return w, w.data_ptr(), need.value
+
+    def _stream(self):
+        return self._torch.cuda.current_stream(self._at).cuda_stream
+
+    def _ck(self, rc):
+        if rc != 0:
+            raise RuntimeError("mlease_hip error %d: %s" % (rc, self.L.mlx_last_error(None).decode()))
+
+    # -- lookup -----------------------------------------------------------------------------------
+    def embedding_lookup(self, table, ids, scale: float = 1.0, out=None):
+        """out[t] = scale * table[ids[t]]; ids outside the table (-1) give rows of zeros. table [rows, width], ids [n] int32 / int64."""
+        tp, ld = self._matrix(table, "table")
+        ip, it = self._ids(ids, "ids")
+        rows, width = table.shape
+        out = self._output(out, "out", (ids.shape[0], width), table.dtype)
+        op, ldo = self._matrix(out, "out")
+        self._ck(self.L.mlx_embedding_lookup(self.device, self._stream(), self._types[table.dtype], tp, rows, width, ld, it, ip, ids.shape[0], scale, op, ldo))
+        return out
+
+    def embedding_gradient(self, grad_out, ids, n_rows: int, scale: float = 1.0, out=None, accumulate: bool = False, dtype=None):
+        """grad[v] = scale * (sum of the rows of grad_out whose id is v), [n_rows, width], in grad_out's type or float32 (dtype, or out's).
+        accumulate: added to `out`, whose other rows are not touched. The same inputs give the same bits."""
+        gp, ldg = self._matrix(grad_out, "grad_out")
+        n, width = grad_out.shape
+        ip, it = self._ids(ids, "ids", n)
+        if accumulate and out is None:
+            raise ValueError("accumulate needs out, the gradient to add to")
+        dtype = dtype or (grad_out.dtype if out is None else out.dtype)
+        if dtype not in self._types:
+            raise ValueError("grad must be of grad_out's type or float32, not %s" % dtype)
+        out = self._output(out, "out", (n_rows, width), dtype)
+        op, ldo = self._matrix(out, "out")
+        keep, wp, wb = self._workspace(self.L.mlx_embedding_gradient_workspace, n_rows, width, n)
+        self._ck(self.L.mlx_embedding_gradient(self.device, self._stream(), self._types[grad_out.dtype], gp, ldg, it, ip, n, scale, bool(accumulate),
+                                               self._types[dtype], op, n_rows, width, ldo, wp, wb))
+        return out
+
+    # -- log-likelihood ---------------------------------------------------------------------------
+    def token_loglik(self, logits, target):
+        """logp[t] = logits[t, target[t]] - log sum exp logits[t] (float32), and stats [n, 2] for token_loglik_gradient. A target outside
+        the classes (-1) is absent: logp 0, and its row is not read."""
+        lp, ld = self._matrix(logits, "logits")
+        n, classes = logits.shape
+        ip, it = self._ids(target, "target", n)
+        f32 = self._torch.float32
+        logp, stats = self._output(None, "logp", (n,), f32), self._output(None, "stats", (n, 2), f32)
+        keep, wp, wb = self._workspace(self.L.mlx_token_loglik_workspace, n, classes)
+        self._ck(self.L.mlx_token_loglik(self.device, self._stream(), self._types[logits.dtype], lp, n, classes, ld, it, ip, logp.data_ptr(), stats.data_ptr(), wp, wb))
+        return logp, stats
+
+    def token_loglik_gradient(self, logits, target, stats, grad_logp, out=None):
+        """dlogits[t, j] = grad_logp[t] * ([j == target[t]] - softmax(logits[t])[j]) in logits' type; out may be logits itself."""
+        lp, ld = self._matrix(logits, "logits")
+        n, classes = logits.shape
+        ip, it = self._ids(target, "target", n)
+        f32 = self._torch.float32
+        gp = self._vector(grad_logp, "grad_logp", n, f32)
+        if tuple(stats.shape) != (n, 2) or not stats.is_contiguous():
+            raise ValueError("stats must be what token_loglik gave for these logits, [%d, 2]" % n)
+        sp = self._vector(stats.view(-1), "stats", 2 * n, f32)
+        out = self._output(out, "out", (n, classes), logits.dtype)
+        op, ldo = self._matrix(out, "out")
+        self._ck(self.L.mlx_token_loglik_gradient(self.device, self._stream(), self._types[logits.dtype], lp, n, classes, ld, it, ip, sp, gp, op, ldo))
+        return out
+
+    # -- preference -------------------------------------------------------------------------------
+    def preference_loss(self, logp, ref_logp, seq_ptr, beta: float = 0.1, smoothing: float = 0.0, scale: float = 1.0, mask=None, weight=None, offset=None,
+                        mean: bool = False, grad: bool = True):
+        """Loss and gradient of pairs of packed sequences: sequence s holds the tokens seq_ptr[s] .. seq_ptr[s + 1], the first half of the sequences
+        are the preferred ones. logp, ref_logp (or None) [n] float32, seq_ptr [2 pairs + 1] int64, mask (or None) [n] bool / uint8, weight, offset
+        (or None) [pairs] float32. Returns loss = sum of scale * weight * pair_loss, pair_loss, margin [pairs], ratio [2 pairs] and grad [n]
+        (None where grad=False)."""
+        torch, f32 = self._torch, self._torch.float32
+        if seq_ptr.dim() != 1 or seq_ptr.shape[0] % 2 != 1:
+            raise ValueError("seq_ptr must be a vector of 2 * pairs + 1 int64, not %s" % (tuple(seq_ptr.shape),))
+        n, pairs = logp.numel(), (seq_ptr.shape[0] - 1) // 2
+        lp, qp = self._vector(logp, "logp", n, f32), self._vector(seq_ptr, "seq_ptr", 2 * pairs + 1, torch.int64)
+        rp = None if ref_logp is None else self._vector(ref_logp, "ref_logp", n, f32)
+        mp = None if mask is None else self._vector(mask, "mask", n, torch.uint8 if mask.dtype == torch.uint8 else torch.bool)
+        wp = None if weight is None else self._vector(weight, "weight", pairs, f32)
+        fp = None if offset is None else self._vector(offset, "offset", pairs, f32)
+        loss, pair_loss, margin = self._output(None, "loss", (), f32), self._output(None, "pair_loss", (pairs,), f32), self._output(None, "margin", (pairs,), f32)
+        ratio, g = self._output(None, "ratio", (2 * pairs,), f32), self._output(None, "grad", (n,), f32) if grad else None
+        keep, kp, kb = self._workspace(self.L.mlx_preference_loss_workspace, n, pairs)
+        self._ck(self.L.mlx_preference_loss(self.device, self._stream(), lp, rp, n, qp, pairs, beta, smoothing, scale, bool(mean), mp, wp, fp, loss.data_ptr(),
+                                            pair_loss.data_ptr(), margin.data_ptr(), ratio.data_ptr(), None if g is None else g.data_ptr(), kp, kb))
+        return PreferenceResult(loss, pair_loss, margin, ratio, g)
