@@ -99,155 +99,388 @@ __global__ __launch_bounds__(256) void k_embedding_lookup(const T *__restrict__ 
 }
 
 // ---------------------------------------------------------------------------------------------- gradient of the lookup
-// The entries are sorted by id (stable, so that equal ids keep ascending t), the sorted list is cut into pieces of SEG entries, a
-// wave sums the rows of a piece for its columns, and sums of an id that crosses a piece's border are joined in the order of the pieces.
-constexpr int RADIX_BITS = 8, RADIX = 1 << RADIX_BITS, SORT_TILE = 2048, SEG = 32;
+// The entries are sorted by id (stable, so that equal ids keep ascending t), then sums run over the sorted list.
+//
+// Sort: least significant digit first, 9 bits a pass, absent entries (key n_rows) last. A workgroup owns a tile of consecutive entries
+// of the list; at most SORT_TILES tiles, so that every workgroup of a pass can add up the other tiles' counts by itself. A pass counts
+// the digits of the next one for the tile an entry goes to, so a pass is one launch. Lists of one tile sort in one launch, in LDS.
+constexpr int DIGIT_BITS = 9, DIGITS = 1 << DIGIT_BITS, SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_TILES = 128;
+constexpr int64_t SORT_TILE = 2048, ONE_TILE = 4096;
 
-struct SortBuf { uint32_t *key[2], *pos[2], *hist; float *part; };
+struct SortPlan { int64_t tile; int tiles, passes; };
 
-template <class I>
-__global__ __launch_bounds__(256) void k_sort_keys(const I *__restrict__ ids, int64_t n, int64_t n_rows, uint32_t *__restrict__ key, uint32_t *__restrict__ pos)
+// lanes of the wave with the same digit
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool here)
 {
-    for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < n; t += gridDim.x * 256ll) {
-        const int64_t id = id_at(ids, t, n_rows);
-        key[t] = (uint32_t)(id < 0 ? n_rows : id);          // absent entries behind all others
-        pos[t] = (uint32_t)t;
+    uint64_t same = __ballot(here);
+#pragma unroll
+    for (int b = 0; b < DIGIT_BITS; b++) {
+        const bool on = (digit >> b) & 1;
+        const uint64_t m = __ballot(on);
+        same &= on ? m : ~m;
+    }
+    return same;
+}
+// exclusive prefix sum over the workgroup's SORT_THREADS = DIGITS values
+__device__ __forceinline__ uint32_t digits_before(uint32_t v, uint32_t *waves)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 63) waves[wave] = x;
+    __syncthreads();
+    uint32_t before = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; w++)
+        if (w < wave) before += waves[w];
+    __syncthreads();
+    return before + x - v;
+}
+template <class I> __device__ __forceinline__ uint32_t key_at(const I *ids, int64_t t, int64_t n_rows)
+{
+    const int64_t id = id_at(ids, t, n_rows);
+    return (uint32_t)(id < 0 ? n_rows : id);
+}
+
+// rows [0, n_rows) of grad to zero by workgroups part, part + parts, ... : 16-byte stores, the whole matrix as one row where it is dense
+template <class G>
+__device__ __forceinline__ void fill_zero(G *grad, int64_t n_rows, int64_t width, int64_t ld, int64_t part, int64_t parts)
+{
+    constexpr int E = Chunk<G>::N;
+    const float zero[E] = {};
+    if (ld == width) { width *= n_rows; n_rows = 1; }
+    const int64_t chunks = width / E, slots = chunks + width % E, step = 4 * SORT_THREADS, cuts = (slots + step - 1) / step;
+    for (int64_t b = part; b < cuts * n_rows; b += parts) {
+        G *row = grad + (b / cuts) * ld;
+        const int64_t first = (b % cuts) * step + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t s = first + i * SORT_THREADS;
+            if (s < chunks) store_chunk(row + s * E, zero);
+            else if (s < slots) row[chunks * E + (s - chunks)] = from_float<G>(0.0f);
+        }
     }
 }
-__global__ __launch_bounds__(256) void k_sort_count(const uint32_t *__restrict__ key, int64_t n, int shift, uint32_t *__restrict__ hist, int nb)
+
+// First launch: the first digit's counts of every tile (workgroups 0 .. tiles - 1), the later passes' counts to zero, and a share of the
+// rows' zeros. counts: [passes][tiles][DIGITS].
+template <class G, class I>
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_begin(const I *__restrict__ ids, int64_t n, int64_t n_rows, SortPlan plan, uint32_t *__restrict__ counts,
+                                                             G *__restrict__ grad, int64_t zero_rows, int64_t width, int64_t ld)
 {
-    __shared__ uint32_t cnt[RADIX];
+    __shared__ uint32_t cnt[DIGITS];
+    if ((int)blockIdx.x >= plan.tiles) {
+        fill_zero(grad, zero_rows, width, ld, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
+        return;
+    }
     cnt[threadIdx.x] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * SORT_TILE;
-    for (int i = threadIdx.x; i < SORT_TILE; i += 256)
-        if (base + i < n) atomicAdd(&cnt[(key[base + i] >> shift) & (RADIX - 1)], 1u);
+    const int64_t lo = (int64_t)blockIdx.x * plan.tile, hi = lo + plan.tile < n ? lo + plan.tile : n;
+    for (int64_t t = lo + threadIdx.x; t < hi; t += SORT_THREADS) atomicAdd(&cnt[key_at(ids, t, n_rows) & (DIGITS - 1)], 1u);
     __syncthreads();
-    hist[(int64_t)threadIdx.x * nb + blockIdx.x] = cnt[threadIdx.x];
+    counts[(int64_t)blockIdx.x * DIGITS + threadIdx.x] = cnt[threadIdx.x];
+    for (int p = 1; p < plan.passes; p++) counts[((int64_t)p * plan.tiles + blockIdx.x) * DIGITS + threadIdx.x] = 0;
 }
-// exclusive prefix sums of hist[0 .. m)
-__global__ __launch_bounds__(1024) void k_sort_scan(uint32_t *__restrict__ hist, int64_t m)
+
+// One pass: the entries of a tile to their places. FIRST: entries come from ids, else from key / pos. The waves of a workgroup take
+// consecutive parts of its tile, 64 entries at a time, so that equal digits keep their order.
+template <class G, class I, bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_pass(const I *__restrict__ ids, int64_t n, int64_t n_rows, SortPlan plan, int pass, uint32_t *__restrict__ counts,
+                                                            const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, uint32_t *__restrict__ key_out,
+                                                            uint32_t *__restrict__ pos_out, G *__restrict__ grad, int64_t zero_rows, int64_t width, int64_t ld)
 {
-    __shared__ uint32_t wsum[16];
-    uint32_t carry = 0;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t b = 0; b < m; b += 1024) {
-        const int64_t i = b + threadIdx.x;
-        const uint32_t v = i < m ? hist[i] : 0;
-        uint32_t x = v;
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t y = __shfl_up(x, d);
-            if (lane >= d) x += y;
+    __shared__ uint32_t at[SORT_WAVES][DIGITS], waves[SORT_WAVES];
+    if ((int)blockIdx.x >= plan.tiles) {
+        fill_zero(grad, zero_rows, width, ld, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, shift = pass * DIGIT_BITS;
+    for (int w = 0; w < SORT_WAVES; w++) at[w][threadIdx.x] = 0;
+    // this thread's digit: entries of it in the tiles before, and in all
+    uint32_t before = 0, all = 0;
+    {
+        const uint32_t *c = counts + (int64_t)pass * plan.tiles * DIGITS + threadIdx.x;
+#pragma unroll 8
+        for (int b = 0; b < plan.tiles; b++) {
+            const uint32_t v = c[(int64_t)b * DIGITS];
+            before += b < (int)blockIdx.x ? v : 0;
+            all += v;
         }
-        if (lane == 63) wsum[wave] = x;
-        __syncthreads();
-        uint32_t before = 0, all = 0;
-        for (int w = 0; w < 16; w++) {
-            if (w < wave) before += wsum[w];
-            all += wsum[w];
+    }
+    const uint32_t first = digits_before(all, waves) + before;       // (synchronises: `at` is zero behind it)
+    const int64_t part = plan.tile / SORT_WAVES, end = (int64_t)(blockIdx.x + 1) * plan.tile < n ? (int64_t)(blockIdx.x + 1) * plan.tile : n;
+    const int64_t lo = (int64_t)blockIdx.x * plan.tile + wave * part, hi = lo + part < end ? lo + part : end;
+    auto entry = [&](int64_t i) { return FIRST ? key_at(ids, i, n_rows) : key[i]; };
+    for (int64_t i = lo + lane; i < hi; i += 64) atomicAdd(&at[wave][(entry(i) >> shift) & (DIGITS - 1)], 1u);
+    __syncthreads();
+    uint32_t run = first;
+    for (int w = 0; w < SORT_WAVES; w++) {
+        const uint32_t c = at[w][threadIdx.x];
+        at[w][threadIdx.x] = run;
+        run += c;
+    }
+    __syncthreads();
+    uint32_t *next = pass + 1 < plan.passes ? counts + (int64_t)(pass + 1) * plan.tiles * DIGITS : nullptr;
+    for (int64_t r = lo; r < hi; r += 64) {
+        const int64_t i = r + lane;
+        const bool here = i < hi;
+        const uint32_t k = here ? entry(i) : 0, p = here ? (FIRST ? (uint32_t)i : pos[i]) : 0, digit = (k >> shift) & (DIGITS - 1);
+        const uint64_t same = same_digit(digit, here);
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        const uint32_t to = at[wave][digit] + rank;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // all lanes have read before the first of a digit moves its counter on
+        if (here && rank == 0) at[wave][digit] += (uint32_t)__popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (here) {
+            key_out[to] = k;
+            pos_out[to] = p;
+            if (next) atomicAdd(&next[(int64_t)(to / (uint32_t)plan.tile) * DIGITS + ((k >> (shift + DIGIT_BITS)) & (DIGITS - 1))], 1u);
         }
-        if (i < m) hist[i] = carry + before + x - v;
-        carry += all;
-        __syncthreads();
     }
 }
-// stable: the four waves of a workgroup take consecutive quarters of its tile, 64 entries at a time
-__global__ __launch_bounds__(256) void k_sort_move(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int64_t n, int shift,
-                                                   const uint32_t *__restrict__ hist, int nb, uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out)
+
+// Lists of up to ONE_TILE entries: workgroup 0 sorts them in LDS, the others write zeros.
+template <class G, class I>
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_one_tile(const I *__restrict__ ids, int n, int64_t n_rows, int passes, uint32_t *__restrict__ key_out,
+                                                                uint32_t *__restrict__ pos_out, G *__restrict__ grad, int64_t zero_rows, int64_t width, int64_t ld)
 {
-    __shared__ uint32_t at[4][RADIX];
+    constexpr int ROUNDS = (int)(ONE_TILE / SORT_THREADS);
+    __shared__ uint32_t at[SORT_WAVES][DIGITS], waves[SORT_WAVES], lkey[ONE_TILE];
+    __shared__ uint16_t lpos[ONE_TILE];
+    if (blockIdx.x > 0) {
+        fill_zero(grad, zero_rows, width, ld, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < 4 * RADIX; i += 256) (&at[0][0])[i] = 0;
-    __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * SORT_TILE + (int64_t)wave * (SORT_TILE / 4);
-    for (int r = 0; r < SORT_TILE / 4; r += 64)
-        if (base + r + lane < n) atomicAdd(&at[wave][(key[base + r + lane] >> shift) & (RADIX - 1)], 1u);
-    __syncthreads();
-    {
-        uint32_t run = hist[(int64_t)threadIdx.x * nb + blockIdx.x];
-        for (int w = 0; w < 4; w++) {
+    const int rounds = (n + SORT_THREADS - 1) / SORT_THREADS, lo = wave * rounds * 64;       // a wave's entries: lo .. lo + rounds * 64
+    uint32_t k[ROUNDS], p[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) {
+        const int i = lo + r * 64 + lane;
+        k[r] = r < rounds && i < n ? key_at(ids, i, n_rows) : 0;
+        p[r] = i;
+    }
+    for (int pass = 0; pass < passes; pass++) {
+        const int shift = pass * DIGIT_BITS;
+        for (int w = 0; w < SORT_WAVES; w++) at[w][threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++)
+            if (r < rounds && lo + r * 64 + lane < n) atomicAdd(&at[wave][(k[r] >> shift) & (DIGITS - 1)], 1u);
+        __syncthreads();
+        uint32_t all = 0;
+        for (int w = 0; w < SORT_WAVES; w++) all += at[w][threadIdx.x];
+        uint32_t run = digits_before(all, waves);
+        for (int w = 0; w < SORT_WAVES; w++) {
             const uint32_t c = at[w][threadIdx.x];
             at[w][threadIdx.x] = run;
             run += c;
         }
-    }
-    __syncthreads();
-    for (int r = 0; r < SORT_TILE / 4; r += 64) {
-        const int64_t i = base + r + lane;
-        const bool here = i < n;
-        const uint32_t k = here ? key[i] : 0, p = here ? pos[i] : 0;
-        const uint32_t digit = (k >> shift) & (RADIX - 1);
-        uint64_t same = __ballot(here);
-        for (int b = 0; b < RADIX_BITS; b++) {
-            const uint64_t m = __ballot((digit >> b) & 1);
-            same &= ((digit >> b) & 1) ? m : ~m;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            if (r >= rounds) break;
+            const bool here = lo + r * 64 + lane < n;
+            const uint32_t digit = (k[r] >> shift) & (DIGITS - 1);
+            const uint64_t same = same_digit(digit, here);
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            const uint32_t to = at[wave][digit] + rank;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (here && rank == 0) at[wave][digit] += (uint32_t)__popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (here) { lkey[to] = k[r]; lpos[to] = (uint16_t)p[r]; }
         }
-        const int before = __popcll(same & ((1ull << lane) - 1));
-        uint32_t to = 0;
-        if (here) to = at[wave][digit] + before;
-        __builtin_amdgcn_wave_barrier();
-        __threadfence_block();
-        if (here && before == 0) at[wave][digit] += (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
-        __threadfence_block();
-        if (here) { key_out[to] = k; pos_out[to] = p; }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const int i = lo + r * 64 + lane;
+            if (r < rounds && i < n) { k[r] = lkey[i]; p[r] = lpos[i]; }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) {
+        const int i = lo + r * 64 + lane;
+        if (r < rounds && i < n) { key_out[i] = k[r]; pos_out[i] = p[r]; }
     }
 }
 
-template <class G>
-__global__ __launch_bounds__(256) void k_rows_zero(G *__restrict__ grad, int64_t n_rows, int64_t width, int64_t ld)
+// Sums. 2^lpr lanes take the columns of a tile (a lane one slot: a 16-byte chunk of grad_out's type, or one of the row's last elements),
+// and a group of lanes adds up the rows of SEG sorted entries. Ids that begin and end inside a group's entries are written at once;
+// the others meet in LDS, where the group in which an id begins adds what the following ones have of it; ids that cross the borders of a
+// workgroup's entries leave a sum before (part[0]) and behind (part[1]) the border for k_piece_join. Always ascending: the same bits.
+constexpr int SEG = 16;
+
+template <class G, int E> __device__ __forceinline__ void put_sum(G *p, const float (&sum)[E], int count, float scale, bool add)
 {
-    const int64_t parts = (width + 255) / 256;
-    for (int64_t b = blockIdx.x; b < n_rows * parts; b += gridDim.x) {
-        const int64_t v = b / parts, j = (b % parts) * 256 + threadIdx.x;
-        if (j < width) grad[v * ld + j] = from_float<G>(0.0f);
-    }
-}
-template <class G> __device__ __forceinline__ void grad_put(G *p, float sum, float scale, bool add)
-{
-    const float x = sum * scale;
-    *p = from_float<G>(add ? to_float(*p) + x : x);
-}
-// one wave per (piece, 64 columns)
-template <class T, class G>
-__global__ __launch_bounds__(64) void k_piece_sums(const T *__restrict__ gout, int64_t ldg, const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
-                                                   int64_t n, float scale, bool add, G *__restrict__ grad, int64_t n_rows, int64_t width, int64_t ld,
-                                                   float *__restrict__ part, int64_t tiles, int64_t pieces)
-{
-    for (int64_t b = blockIdx.x; b < pieces * tiles; b += gridDim.x) {
-        const int64_t c = b / tiles, j = (b % tiles) * 64 + threadIdx.x;
-        const int64_t lo = c * SEG, hi = lo + SEG < n ? lo + SEG : n;
-        if (j >= width) continue;
-        const int64_t before = c ? (int64_t)key[lo - 1] : -1, after = hi < n ? (int64_t)key[hi] : -1;
-        float sum = 0.0f;
-        bool first = true;                       // the piece's first id: it may have begun in the piece before
-        for (int64_t i = lo; i < hi; i++) {
-            const int64_t k = key[i];
-            if (k >= n_rows) break;
-            sum += to_float(gout[(int64_t)pos[i] * ldg + j]);
-            if (i + 1 < hi && (int64_t)key[i + 1] == k) continue;
-            if (first && before == k) part[(2 * c) * width + j] = sum;
-            else if (i + 1 == hi && after == k) part[(2 * c + 1) * width + j] = sum;
-            else grad_put(grad + k * ld + j, sum, scale, add);
-            sum = 0.0f;
-            first = false;
+#pragma unroll
+    for (int i = 0; i < E; i++)
+        if (i < count) {
+            const float x = sum[i] * scale;
+            p[i] = from_float<G>(add ? to_float(p[i]) + x : x);
         }
+}
+template <class G, int E> __device__ __forceinline__ void put_slot(G *p, const float (&sum)[E], bool vec, float scale, bool add)
+{
+    if (!vec) { put_sum<G, E>(p, sum, 1, scale, add); return; }
+    constexpr int EG = Chunk<G>::N;          // E of grad_out's type are one or two chunks of grad's
+#pragma unroll
+    for (int c = 0; c < E / EG; c++) {
+        float f[EG] = {};
+        if (add) load_chunk(p + c * EG, f);
+#pragma unroll
+        for (int i = 0; i < EG; i++) f[i] = add ? f[i] + sum[c * EG + i] * scale : sum[c * EG + i] * scale;
+        store_chunk(p + c * EG, f);
     }
 }
-// an id that begins in piece c and goes on in the next ones: its sums in the order of the pieces
-template <class G>
-__global__ __launch_bounds__(64) void k_piece_join(const uint32_t *__restrict__ key, int64_t n, float scale, bool add, G *__restrict__ grad, int64_t n_rows,
-                                                   int64_t width, int64_t ld, const float *__restrict__ part, int64_t tiles, int64_t pieces)
+
+struct SumArgs {
+    const uint32_t *key, *pos;
+    int64_t n, n_rows, width, ldg, ld, slots, tiles, pieces;
+    float scale;
+    int add, lpr;
+    float *part;                             // [pieces][2][slots][E]
+};
+
+template <class T, class G>
+__global__ __launch_bounds__(256) void k_piece_sums(const T *__restrict__ gout, G *__restrict__ grad, SumArgs a)
 {
-    for (int64_t b = blockIdx.x; b < pieces * tiles; b += gridDim.x) {
-        const int64_t c = b / tiles, j = (b % tiles) * 64 + threadIdx.x;
-        const int64_t lo = c * SEG, hi = lo + SEG;
-        if (j >= width || hi >= n) continue;
-        const int64_t k = key[hi - 1];
-        if (k >= n_rows || (int64_t)key[hi] != k || (c && (int64_t)key[lo - 1] == k)) continue;
-        float sum = part[(2 * c + 1) * width + j];
-        for (int64_t d = c + 1; d < pieces && (int64_t)key[d * SEG] == k; d++) sum += part[(2 * d) * width + j];
-        grad_put(grad + k * ld + j, sum, scale, add);
+    constexpr int E = Chunk<T>::N;
+    __shared__ float head[256][E], tail[256][E];
+    __shared__ uint8_t kind[256];            // per group: 1 its first id began before it, 2 that id goes on behind it, 4 its last id begins here and goes on
+    const int lane = threadIdx.x & ((1 << a.lpr) - 1), group = threadIdx.x >> a.lpr, groups = 256 >> a.lpr;
+    const int64_t per = (int64_t)groups * SEG;
+    for (int64_t b = blockIdx.x; b < a.pieces * a.tiles; b += gridDim.x) {
+        const int64_t piece = b / a.tiles, slot = ((b % a.tiles) << a.lpr) + lane;
+        const int64_t lo = piece * per + group * SEG;
+        const int64_t chunks = a.width / E;
+        const bool vec = slot < chunks, mine = slot < a.slots;
+        const int64_t j = vec ? slot * E : chunks * E + (slot - chunks);
+        uint32_t k[SEG], p[SEG];
+#pragma unroll
+        for (int i = 0; i < SEG; i++) {
+            const bool in = lo + i < a.n;
+            k[i] = in ? a.key[lo + i] : (uint32_t)a.n_rows;
+            p[i] = in ? a.pos[lo + i] : 0;
+        }
+        const uint32_t before = lo > 0 && lo < a.n ? a.key[lo - 1] : 0xffffffffu, after = lo + SEG < a.n ? a.key[lo + SEG] : 0xffffffffu;
+        int what = 0;
+        uint32_t last = 0;
+        float sum[E] = {};
+        bool first = true;
+#pragma unroll
+        for (int i0 = 0; i0 < SEG; i0 += 8) {
+            float f[8][E];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+#pragma unroll
+                for (int e = 0; e < E; e++) f[i][e] = 0.0f;
+                if (mine && k[i0 + i] < (uint32_t)a.n_rows) {
+                    const T *row = gout + (int64_t)p[i0 + i] * a.ldg + j;
+                    if (vec) load_chunk(row, f[i]);
+                    else f[i][0] = to_float(row[0]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t key = k[i0 + i];
+                if (key >= (uint32_t)a.n_rows) continue;             // absent entries, and those behind the list, are last
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] += f[i][e];
+                const bool end = i0 + i == SEG - 1;
+                const uint32_t next = end ? after : k[(i0 + i + 1) & (SEG - 1)];
+                if (!end && next == key) continue;
+                if (first && before == key) {
+                    what |= end && next == key ? 3 : 1;
+#pragma unroll
+                    for (int e = 0; e < E; e++) head[threadIdx.x][e] = sum[e];
+                } else if (end && next == key) {
+                    what |= 4;
+                    last = key;
+#pragma unroll
+                    for (int e = 0; e < E; e++) tail[threadIdx.x][e] = sum[e];
+                } else if (mine) put_slot<G, E>(grad + (int64_t)key * a.ld + j, sum, vec, a.scale, a.add);
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] = 0.0f;
+                first = false;
+            }
+        }
+        if (lane == 0) kind[group] = (uint8_t)what;
+        __syncthreads();
+        // an id that begins in this group (its tail), and in group 0 also the one that began before the workgroup's entries
+        for (int side = group == 0 ? 0 : 1; side < 2; side++) {
+            if (side == 0 ? !(what & 1) : !(what & 4)) continue;
+            int q = side == 0 ? 0 : group + 1;
+            bool on = side == 0 ? (what & 2) : true;                 // goes on behind group q (side 0) or into it (side 1)
+#pragma unroll
+            for (int e = 0; e < E; e++) sum[e] = side == 0 ? head[threadIdx.x][e] : tail[threadIdx.x][e];
+            if (side == 0) q = 1;
+            while (on && q < groups) {
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] += head[(q << a.lpr) + lane][e];
+                on = kind[q] & 2;
+                q++;
+            }
+            if (!mine) continue;
+            if (side == 0 || on) {
+                float *out = a.part + ((piece * 2 + side) * a.slots + slot) * E;
+#pragma unroll
+                for (int e = 0; e < E; e++) out[e] = sum[e];
+            } else put_slot<G, E>(grad + (int64_t)last * a.ld + j, sum, vec, a.scale, a.add);
+        }
+        __syncthreads();
+    }
+}
+
+// Ids that cross the border of two pieces: the workgroup of the piece in which one begins adds its sums in the order of the pieces,
+// its groups of lanes consecutive parts of them.
+template <class T, class G>
+__global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArgs a)
+{
+    constexpr int E = Chunk<T>::N;
+    __shared__ float sums[256][E];
+    const int lane = threadIdx.x & ((1 << a.lpr) - 1), group = threadIdx.x >> a.lpr, groups = 256 >> a.lpr;
+    const int64_t per = (int64_t)groups * SEG;
+    for (int64_t b = blockIdx.x; b < (a.pieces - 1) * a.tiles; b += gridDim.x) {
+        const int64_t piece = b / a.tiles, slot = ((b % a.tiles) << a.lpr) + lane, lo = piece * per, hi = lo + per;       // hi < n
+        const uint32_t k = a.key[hi - 1];
+        if (k >= (uint32_t)a.n_rows || a.key[hi] != k || (piece && a.key[lo - 1] == k)) continue;
+        // the last piece whose first entry has this id
+        int64_t x = piece + 1, y = a.pieces;
+        while (y - x > 1) {
+            const int64_t m = (x + y) / 2;
+            if (a.key[m * per] == k) x = m;
+            else y = m;
+        }
+        const int64_t count = x - piece, share = (count + groups - 1) / groups;          // sums of pieces piece + 1 .. x, and the tail of `piece`
+        const int64_t from = piece + 1 + group * share, to = from + share < x + 1 ? from + share : x + 1;
+        const bool mine = slot < a.slots;
+        float sum[E] = {};
+        if (mine) {
+            if (group == 0)
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] = a.part[((piece * 2 + 1) * a.slots + slot) * E + e];
+#pragma unroll 4
+            for (int64_t q = from; q < to; q++)
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] += a.part[((q * 2) * a.slots + slot) * E + e];
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) sums[threadIdx.x][e] = sum[e];
+        __syncthreads();
+        if (group == 0 && mine) {
+            for (int q = 1; q < groups; q++)
+#pragma unroll
+                for (int e = 0; e < E; e++) sum[e] += sums[(q << a.lpr) + lane][e];
+            const int64_t chunks = a.width / E;
+            const bool vec = slot < chunks;
+            put_slot<G, E>(grad + (int64_t)k * a.ld + (vec ? slot * E : chunks * E + (slot - chunks)), sum, vec, a.scale, a.add);
+        }
+        __syncthreads();
     }
 }
 
@@ -474,17 +707,25 @@ int check_matrix(const char *who, const char *what, const void *p, int64_t rows,
     return MLX_OK;
 }
 
-struct GradientPlan { size_t key, hist, part, bytes; int64_t nb, pieces; };
-GradientPlan gradient_plan(int64_t width, int64_t n)
+struct GradientPlan { SortPlan sort; int lpr; int64_t slots, tiles, pieces; size_t key, counts, part, bytes; };
+GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
 {
     GradientPlan g;
-    g.nb = ceil_div(n, SORT_TILE);
-    g.pieces = ceil_div(n, SEG);
+    const int64_t E = 16 / es;
+    g.sort.tile = n <= ONE_TILE ? ONE_TILE : std::max(SORT_TILE, ceil_div(ceil_div(n, SORT_TILES), SORT_THREADS) * SORT_THREADS);
+    g.sort.tiles = (int)ceil_div(n, g.sort.tile);
+    g.sort.passes = 1;
+    while (n_rows >> (g.sort.passes * DIGIT_BITS)) g.sort.passes++;          // keys run from 0 to n_rows
+    g.slots = width / E + width % E;
+    g.lpr = 0;
+    while (g.lpr < 6 && (1 << g.lpr) < g.slots) g.lpr++;
+    g.tiles = ceil_div(g.slots, 1 << g.lpr);
+    g.pieces = ceil_div(n, (int64_t)(256 >> g.lpr) * SEG);
     auto round = [](size_t b) { return (b + 255) / 256 * 256; };
     g.key = round((size_t)n * 4);
-    g.hist = round((size_t)g.nb * RADIX * 4);
-    g.part = round((size_t)g.pieces * 2 * (size_t)width * 4);
-    g.bytes = 4 * g.key + g.hist + g.part;
+    g.counts = n <= ONE_TILE ? 0 : round((size_t)g.sort.passes * g.sort.tiles * DIGITS * 4);
+    g.part = g.pieces > 1 ? round((size_t)g.pieces * 2 * (size_t)g.slots * (size_t)E * 4) : 0;
+    g.bytes = 4 * g.key + g.counts + g.part;
     return g;
 }
 
@@ -530,7 +771,7 @@ int mlx_embedding_gradient_workspace(int64_t n_rows, int64_t width, int64_t n_id
     const char *who = "mlx_embedding_gradient_workspace";
     MLX_REFUSE(!bytes, "%s: bytes is NULL", who);
     MLX_REFUSE(n_rows < 0 || n_rows > MOST || n_ids < 0 || n_ids > MOST || width < 1 || width > MOST, "%s: bad sizes", who);
-    *bytes = gradient_plan(width, n_ids).bytes;
+    *bytes = std::max(gradient_plan(4, n_rows, width, n_ids).bytes, gradient_plan(2, n_rows, width, n_ids).bytes);
     return MLX_OK;
 }
 
@@ -547,7 +788,7 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
     int rc;
     if ((rc = check_matrix(who, "grad_out", grad_out, n_ids, width, ld_grad_out, es, false)) || (rc = check_matrix(who, "grad", grad, n_rows, width, ld_grad, gs, true))) return rc;
     MLX_REFUSE(n_ids > 0 && (!ids || (uintptr_t)ids % (uintptr_t)is), "%s: ids is NULL or not aligned", who);
-    const GradientPlan plan = gradient_plan(width, n_ids);
+    const GradientPlan plan = gradient_plan(es, n_rows, width, n_ids);
     MLX_REFUSE(workspace_bytes < plan.bytes, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, plan.bytes);
     MLX_REFUSE(plan.bytes && (!workspace || (uintptr_t)workspace % 256), "%s: workspace is NULL or not aligned to 256 bytes", who);
     const int64_t gb = span(n_rows, width, ld_grad, gs);
@@ -558,33 +799,53 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
     if (on.rc) return on.rc;
     hipStream_t st = (hipStream_t)stream;
     char *w = (char *)workspace;
-    SortBuf sb;
-    sb.key[0] = (uint32_t *)w; sb.key[1] = (uint32_t *)(w + plan.key); sb.pos[0] = (uint32_t *)(w + 2 * plan.key); sb.pos[1] = (uint32_t *)(w + 3 * plan.key);
-    sb.hist = (uint32_t *)(w + 4 * plan.key); sb.part = (float *)(w + 4 * plan.key + plan.hist);
+    uint32_t *key[2] = { (uint32_t *)w, (uint32_t *)(w + plan.key) }, *pos[2] = { (uint32_t *)(w + 2 * plan.key), (uint32_t *)(w + 3 * plan.key) };
+    uint32_t *counts = (uint32_t *)(w + 4 * plan.key);
+    float *part = (float *)(w + 4 * plan.key + plan.counts);
     auto with = [&](auto t, auto g) {
         typedef decltype(t) T;
         typedef decltype(g) G;
-        if (!accumulate)
-            hipLaunchKernelGGL((k_rows_zero<G>), dim3(grid_of(n_rows * ceil_div(width, 256))), dim3(256), 0, st, (G *)grad, n_rows, width, ld_grad);
-        if (n_ids == 0) return 0;
-        by_id(id_type, [&](auto i) {
+        return by_id(id_type, [&](auto i) {
             typedef decltype(i) I;
-            hipLaunchKernelGGL((k_sort_keys<I>), dim3(grid_of(ceil_div(n_ids, 256))), dim3(256), 0, st, (const I *)ids, n_ids, n_rows, sb.key[0], sb.pos[0]);
+            const I *id = (const I *)ids;
+            G *out = (G *)grad;
+            // The zeros of grad go along with the sort's launches, each a share of the rows: the few workgroups of the sort run beside them.
+            const int shares = n_ids <= ONE_TILE ? 1 : plan.sort.passes + 1;
+            int64_t row = 0;
+            struct Share { G *at; int64_t rows; unsigned blocks; };
+            auto zeros = [&](int k) {
+                const int64_t end = accumulate ? 0 : n_rows * (k + 1) / shares, rows = end - row;
+                Share s = { out + row * ld_grad, rows, 0 };
+                if (rows > 0) s.blocks = (unsigned)std::min<int64_t>(2048, ceil_div(rows * width, 4 * SORT_THREADS * Chunk<G>::N));
+                row = end;
+                return s;
+            };
+            int cur = 0;
+            if (n_ids <= ONE_TILE) {
+                const Share z = zeros(0);
+                hipLaunchKernelGGL((k_sort_one_tile<G, I>), dim3(1 + z.blocks), dim3(SORT_THREADS), 0, st, id, (int)n_ids, n_rows, plan.sort.passes, key[0], pos[0], z.at, z.rows,
+                                   width, ld_grad);
+            } else {
+                Share z = zeros(0);
+                hipLaunchKernelGGL((k_sort_begin<G, I>), dim3(plan.sort.tiles + z.blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, counts, z.at, z.rows, width,
+                                   ld_grad);
+                for (int pass = 0; pass < plan.sort.passes; pass++) {
+                    z = zeros(pass + 1);
+                    if (pass == 0)
+                        hipLaunchKernelGGL((k_sort_pass<G, I, true>), dim3(plan.sort.tiles + z.blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, pass, counts,
+                                           nullptr, nullptr, key[0], pos[0], z.at, z.rows, width, ld_grad);
+                    else
+                        hipLaunchKernelGGL((k_sort_pass<G, I, false>), dim3(plan.sort.tiles + z.blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, pass, counts,
+                                           key[cur], pos[cur], key[cur ^ 1], pos[cur ^ 1], z.at, z.rows, width, ld_grad);
+                    if (pass) cur ^= 1;
+                }
+            }
+            if (n_ids == 0) return 0;
+            const SumArgs a = { key[cur], pos[cur], n_ids, n_rows, width, ld_grad_out, ld_grad, plan.slots, plan.tiles, plan.pieces, scale, accumulate != 0, plan.lpr, part };
+            hipLaunchKernelGGL((k_piece_sums<T, G>), dim3(grid_of(plan.pieces * plan.tiles)), dim3(256), 0, st, (const T *)grad_out, out, a);
+            if (plan.pieces > 1) hipLaunchKernelGGL((k_piece_join<T, G>), dim3(grid_of((plan.pieces - 1) * plan.tiles)), dim3(256), 0, st, out, a);
             return 0;
         });
-        int cur = 0;
-        for (int shift = 0; shift == 0 || (n_rows >> shift) != 0; shift += RADIX_BITS, cur ^= 1) {      // keys run from 0 to n_rows
-            hipLaunchKernelGGL(k_sort_count, dim3((unsigned)plan.nb), dim3(256), 0, st, sb.key[cur], n_ids, shift, sb.hist, (int)plan.nb);
-            hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, sb.hist, plan.nb * RADIX);
-            hipLaunchKernelGGL(k_sort_move, dim3((unsigned)plan.nb), dim3(256), 0, st, sb.key[cur], sb.pos[cur], n_ids, shift, sb.hist, (int)plan.nb,
-                               sb.key[cur ^ 1], sb.pos[cur ^ 1]);
-        }
-        const int64_t tiles = ceil_div(width, 64);
-        hipLaunchKernelGGL((k_piece_sums<T, G>), dim3(grid_of(plan.pieces * tiles)), dim3(64), 0, st, (const T *)grad_out, ld_grad_out, sb.key[cur], sb.pos[cur], n_ids,
-                           scale, accumulate != 0, (G *)grad, n_rows, width, ld_grad, sb.part, tiles, plan.pieces);
-        hipLaunchKernelGGL((k_piece_join<G>), dim3(grid_of(plan.pieces * tiles)), dim3(64), 0, st, sb.key[cur], n_ids, scale, accumulate != 0, (G *)grad, n_rows, width,
-                           ld_grad, sb.part, tiles, plan.pieces);
-        return 0;
     };
     by_type(type, [&](auto t) { return grad_type == MLX_F32 ? with(t, float()) : with(t, t); });
     return launched(who);
