@@ -38,25 +38,53 @@ template <class T> __device__ __forceinline__ T from_float(float x)
     return (T)x;
 }
 
-template <class T> __device__ __forceinline__ void load_chunk(const T *p, float (&f)[Chunk<T>::N])
+// NT: past the caches' usual replacement, for matrices that do not fit them and are read or written once (the entry points' rule: streams())
+template <bool NT, class T> __device__ __forceinline__ u32x4 load_raw(const T *p)
+{
+    const auto *v = reinterpret_cast<const typename Chunk<T>::vec *>(p);
+    if constexpr (NT) return __builtin_nontemporal_load(v);
+    else return *v;
+}
+template <class T> __device__ __forceinline__ void unpack(u32x4 raw, float *f)
 {
     union { u32x4 v; T e[Chunk<T>::N]; } u;
-    u.v = *reinterpret_cast<const typename Chunk<T>::vec *>(p);
+    u.v = raw;
 #pragma unroll
     for (int i = 0; i < Chunk<T>::N; i++) f[i] = to_float(u.e[i]);
 }
-template <class T> __device__ __forceinline__ void store_chunk(T *p, const float (&f)[Chunk<T>::N])
+template <bool NT, class T> __device__ __forceinline__ void load_chunk(const T *p, float (&f)[Chunk<T>::N]) { unpack<T>(load_raw<NT>(p), f); }
+template <bool NT, class T> __device__ __forceinline__ void store_chunk(T *p, const float (&f)[Chunk<T>::N])
 {
     union { u32x4 v; T e[Chunk<T>::N]; } u;
 #pragma unroll
     for (int i = 0; i < Chunk<T>::N; i++) u.e[i] = from_float<T>(f[i]);
-    *reinterpret_cast<typename Chunk<T>::vec *>(p) = u.v;
+    auto *v = reinterpret_cast<typename Chunk<T>::vec *>(p);
+    if constexpr (NT) __builtin_nontemporal_store(u.v, v);
+    else *v = u.v;
 }
+// A row of at least N elements is cut into slots of N: the last one begins at width - N and holds what the others have not (from `skip` on).
+// Narrower rows are one slot, read and written element by element.
+template <class T> struct Slot {
+    static constexpr int N = Chunk<T>::N;
+    int64_t j;                               // first element
+    int skip, count;                         // the slot's own elements: skip .. skip + count
+    __device__ __forceinline__ Slot(int64_t s, int64_t width)
+    {
+        const int64_t first = s * N;
+        j = first + N <= width ? first : width - N;
+        skip = (int)(first - j);
+        count = N - skip;
+        if (width < N) { j = 0; skip = 0; count = (int)width; }
+    }
+    __device__ __forceinline__ bool whole() const { return count == N; }
+};
+int64_t slots_of(int64_t width, int64_t n) { return (width + n - 1) / n; }
 
-// id of entry t, or -1 where it is outside [0, n)
-template <class I> __device__ __forceinline__ int64_t id_at(const I *ids, int64_t t, int64_t n)
+// ids of either type; id of entry t, or -1 where it is outside [0, n)
+struct Ids { const void *p; int wide; };
+__device__ __forceinline__ int64_t id_at(Ids ids, int64_t t, int64_t n)
 {
-    const int64_t v = (int64_t)ids[t];
+    const int64_t v = ids.wide ? static_cast<const int64_t *>(ids.p)[t] : (int64_t)static_cast<const int32_t *>(ids.p)[t];
     return (v < 0 || v >= n) ? -1 : v;
 }
 
@@ -68,33 +96,32 @@ template <class T, class Op> __device__ __forceinline__ T wave_all(T x, Op op)
 }
 
 // ---------------------------------------------------------------------------------------------- lookup
-// A row is cut into slots: its 16-byte chunks, then its last elements one by one. 2^lpr lanes take a row, 256 >> lpr rows a workgroup.
-template <class T, class I>
-__global__ __launch_bounds__(256) void k_embedding_lookup(const T *__restrict__ table, int64_t n_rows, int64_t width, int64_t ldt, const I *__restrict__ ids,
-                                                          int64_t n, float scale, T *__restrict__ out, int64_t ldo, int lpr, int64_t groups)
+// 2^lpr lanes take a row, a lane every 2^lpr-th slot, 256 >> lpr rows a workgroup.
+template <class T, bool NT, bool NARROW>
+__global__ __launch_bounds__(256) void k_embedding_lookup(const T *__restrict__ table, int64_t n_rows, int64_t width, int64_t ldt, Ids ids, int64_t n, float scale,
+                                                          T *__restrict__ out, int64_t ldo, int lpr, int64_t groups)
 {
     constexpr int E = Chunk<T>::N;
-    const int64_t chunks = width / E, slots = chunks + width % E;
+    const int64_t slots = NARROW ? 1 : (width + E - 1) / E;
     const int lane = threadIdx.x & ((1 << lpr) - 1);
     for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
         const int64_t t = g * (256 >> lpr) + (threadIdx.x >> lpr);
         if (t >= n) continue;
         const int64_t id = id_at(ids, t, n_rows);
-        for (int64_t s = lane; s < slots; s += 1 << lpr) {
-            if (s < chunks) {
+        T *o = out + t * ldo;
+        if constexpr (NARROW) {
+            for (int j = 0; j < (int)width; j++) o[j] = from_float<T>(id < 0 ? 0.0f : to_float(table[id * ldt + j]) * scale);
+        } else
+            for (int64_t s = lane; s < slots; s += 1 << lpr) {
+                const Slot<T> at(s, width);
                 float f[E] = {};
-                if (id >= 0) load_chunk(table + id * ldt + s * E, f);
+                if (id >= 0) {
+                    load_chunk<false>(table + id * ldt + at.j, f);       // rows repeat: through the caches as usual
 #pragma unroll
-                for (int i = 0; i < E; i++) f[i] *= scale;
-                if (id < 0)
-#pragma unroll
-                    for (int i = 0; i < E; i++) f[i] = 0.0f;
-                store_chunk(out + t * ldo + s * E, f);
-            } else {
-                const int64_t j = chunks * E + (s - chunks);
-                out[t * ldo + j] = from_float<T>(id < 0 ? 0.0f : to_float(table[id * ldt + j]) * scale);
+                    for (int i = 0; i < E; i++) f[i] *= scale;
+                }
+                store_chunk<NT>(o + at.j, f);                            // the last slot writes some of its neighbour's elements again, the same values
             }
-        }
     }
 }
 
@@ -140,14 +167,14 @@ __device__ __forceinline__ uint32_t digits_before(uint32_t v, uint32_t *waves)
     __syncthreads();
     return before + x - v;
 }
-template <class I> __device__ __forceinline__ uint32_t key_at(const I *ids, int64_t t, int64_t n_rows)
+__device__ __forceinline__ uint32_t key_at(Ids ids, int64_t t, int64_t n_rows)
 {
     const int64_t id = id_at(ids, t, n_rows);
     return (uint32_t)(id < 0 ? n_rows : id);
 }
 
-// rows [0, n_rows) of grad to zero by workgroups part, part + parts, ... : 16-byte stores, the whole matrix as one row where it is dense
-template <class G>
+// rows [0, n_rows) of grad to zero by workgroups part, part + parts, ... ; the whole matrix as one row where it is dense
+template <class G, bool NT>
 __device__ __forceinline__ void fill_zero(G *grad, int64_t n_rows, int64_t width, int64_t ld, int64_t part, int64_t parts)
 {
     constexpr int E = Chunk<G>::N;
@@ -160,99 +187,118 @@ __device__ __forceinline__ void fill_zero(G *grad, int64_t n_rows, int64_t width
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int64_t s = first + i * SORT_THREADS;
-            if (s < chunks) store_chunk(row + s * E, zero);
+            if (s < chunks) store_chunk<NT>(row + s * E, zero);
             else if (s < slots) row[chunks * E + (s - chunks)] = from_float<G>(0.0f);
         }
     }
 }
+template <class G> struct Zeros { G *grad; int64_t rows, width, ld; };      // the rows a launch writes along
 
-// First launch: the first digit's counts of every tile (workgroups 0 .. tiles - 1), the later passes' counts to zero, and a share of the
-// rows' zeros. counts: [passes][tiles][DIGITS].
-template <class G, class I>
-__global__ __launch_bounds__(SORT_THREADS) void k_sort_begin(const I *__restrict__ ids, int64_t n, int64_t n_rows, SortPlan plan, uint32_t *__restrict__ counts,
-                                                             G *__restrict__ grad, int64_t zero_rows, int64_t width, int64_t ld)
+// Counts of the digits of a pass in every tile, [tiles][DIGITS] (workgroups 0 .. tiles - 1; the others write zeros). FIRST: entries come from
+// ids, else from key.
+template <class G, bool NT, bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_count(Ids ids, int64_t n, int64_t n_rows, SortPlan plan, int shift, uint32_t *__restrict__ counts,
+                                                             const uint32_t *__restrict__ key, Zeros<G> z)
 {
     __shared__ uint32_t cnt[DIGITS];
     if ((int)blockIdx.x >= plan.tiles) {
-        fill_zero(grad, zero_rows, width, ld, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
+        fill_zero<G, NT>(z.grad, z.rows, z.width, z.ld, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
         return;
     }
     cnt[threadIdx.x] = 0;
     __syncthreads();
     const int64_t lo = (int64_t)blockIdx.x * plan.tile, hi = lo + plan.tile < n ? lo + plan.tile : n;
-    for (int64_t t = lo + threadIdx.x; t < hi; t += SORT_THREADS) atomicAdd(&cnt[key_at(ids, t, n_rows) & (DIGITS - 1)], 1u);
+#pragma unroll 4
+    for (int64_t t = lo + threadIdx.x; t < hi; t += SORT_THREADS) atomicAdd(&cnt[((FIRST ? key_at(ids, t, n_rows) : key[t]) >> shift) & (DIGITS - 1)], 1u);
     __syncthreads();
     counts[(int64_t)blockIdx.x * DIGITS + threadIdx.x] = cnt[threadIdx.x];
-    for (int p = 1; p < plan.passes; p++) counts[((int64_t)p * plan.tiles + blockIdx.x) * DIGITS + threadIdx.x] = 0;
 }
 
-// One pass: the entries of a tile to their places. FIRST: entries come from ids, else from key / pos. The waves of a workgroup take
-// consecutive parts of its tile, 64 entries at a time, so that equal digits keep their order.
-template <class G, class I, bool FIRST>
-__global__ __launch_bounds__(SORT_THREADS) void k_sort_pass(const I *__restrict__ ids, int64_t n, int64_t n_rows, SortPlan plan, int pass, uint32_t *__restrict__ counts,
+// One pass: the entries of a tile to their places. The waves of a workgroup take consecutive parts of its tile, 64 entries at a time, so that
+// equal digits keep their order.
+template <class G, bool NT, bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_move(Ids ids, int64_t n, int64_t n_rows, SortPlan plan, int shift, const uint32_t *__restrict__ counts,
                                                             const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, uint32_t *__restrict__ key_out,
-                                                            uint32_t *__restrict__ pos_out, G *__restrict__ grad, int64_t zero_rows, int64_t width, int64_t ld)
+                                                            uint32_t *__restrict__ pos_out, Zeros<G> z)
 {
+    constexpr int AHEAD = 4, COLUMN = 32;
     __shared__ uint32_t at[SORT_WAVES][DIGITS], waves[SORT_WAVES];
     if ((int)blockIdx.x >= plan.tiles) {
-        fill_zero(grad, zero_rows, width, ld, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
+        fill_zero<G, NT>(z.grad, z.rows, z.width, z.ld, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
         return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, shift = pass * DIGIT_BITS;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
     for (int w = 0; w < SORT_WAVES; w++) at[w][threadIdx.x] = 0;
-    // this thread's digit: entries of it in the tiles before, and in all
+    // this thread's digit: entries of it in the tiles before, and in all; COLUMN loads at a time (the last tile again behind the end)
     uint32_t before = 0, all = 0;
-    {
-        const uint32_t *c = counts + (int64_t)pass * plan.tiles * DIGITS + threadIdx.x;
-#pragma unroll 8
-        for (int b = 0; b < plan.tiles; b++) {
-            const uint32_t v = c[(int64_t)b * DIGITS];
-            before += b < (int)blockIdx.x ? v : 0;
-            all += v;
+    for (int b0 = 0; b0 < plan.tiles; b0 += COLUMN) {
+        uint32_t v[COLUMN];
+#pragma unroll
+        for (int b = 0; b < COLUMN; b++) v[b] = counts[(int64_t)(b0 + b < plan.tiles ? b0 + b : plan.tiles - 1) * DIGITS + threadIdx.x];
+#pragma unroll
+        for (int b = 0; b < COLUMN; b++) {
+            before += b0 + b < (int)blockIdx.x ? v[b] : 0;
+            all += b0 + b < plan.tiles ? v[b] : 0;
         }
     }
     const uint32_t first = digits_before(all, waves) + before;       // (synchronises: `at` is zero behind it)
     const int64_t part = plan.tile / SORT_WAVES, end = (int64_t)(blockIdx.x + 1) * plan.tile < n ? (int64_t)(blockIdx.x + 1) * plan.tile : n;
     const int64_t lo = (int64_t)blockIdx.x * plan.tile + wave * part, hi = lo + part < end ? lo + part : end;
-    auto entry = [&](int64_t i) { return FIRST ? key_at(ids, i, n_rows) : key[i]; };
-    for (int64_t i = lo + lane; i < hi; i += 64) atomicAdd(&at[wave][(entry(i) >> shift) & (DIGITS - 1)], 1u);
+    uint32_t k[AHEAD], p[AHEAD];
+    auto fetch = [&](int64_t r, bool places) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int64_t i = r + a * 64 + lane, c = i < hi ? i : hi - 1;
+            k[a] = FIRST ? key_at(ids, c, n_rows) : key[c];
+            if (places) p[a] = FIRST ? (uint32_t)c : pos[c];
+        }
+    };
+    for (int64_t r = lo; r < hi; r += AHEAD * 64) {
+        fetch(r, false);
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++)
+            if (r + a * 64 + lane < hi) atomicAdd(&at[wave][(k[a] >> shift) & (DIGITS - 1)], 1u);
+    }
     __syncthreads();
     uint32_t run = first;
+#pragma unroll
     for (int w = 0; w < SORT_WAVES; w++) {
         const uint32_t c = at[w][threadIdx.x];
         at[w][threadIdx.x] = run;
         run += c;
     }
     __syncthreads();
-    uint32_t *next = pass + 1 < plan.passes ? counts + (int64_t)(pass + 1) * plan.tiles * DIGITS : nullptr;
-    for (int64_t r = lo; r < hi; r += 64) {
-        const int64_t i = r + lane;
-        const bool here = i < hi;
-        const uint32_t k = here ? entry(i) : 0, p = here ? (FIRST ? (uint32_t)i : pos[i]) : 0, digit = (k >> shift) & (DIGITS - 1);
-        const uint64_t same = same_digit(digit, here);
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        const uint32_t to = at[wave][digit] + rank;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // all lanes have read before the first of a digit moves its counter on
-        if (here && rank == 0) at[wave][digit] += (uint32_t)__popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (here) {
-            key_out[to] = k;
-            pos_out[to] = p;
-            if (next) atomicAdd(&next[(int64_t)(to / (uint32_t)plan.tile) * DIGITS + ((k >> (shift + DIGIT_BITS)) & (DIGITS - 1))], 1u);
+    for (int64_t r = lo; r < hi; r += AHEAD * 64) {
+        fetch(r, true);
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const bool here = r + a * 64 + lane < hi;
+            const uint32_t digit = (k[a] >> shift) & (DIGITS - 1);
+            const uint64_t same = same_digit(digit, here);
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            const uint32_t to = at[wave][digit] + rank;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // all lanes have read before the first of a digit moves its counter on
+            if (here && rank == 0) at[wave][digit] += (uint32_t)__popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (here) {
+                key_out[to] = k[a];
+                pos_out[to] = p[a];
+            }
         }
     }
 }
 
 // Lists of up to ONE_TILE entries: workgroup 0 sorts them in LDS, the others write zeros.
-template <class G, class I>
-__global__ __launch_bounds__(SORT_THREADS) void k_sort_one_tile(const I *__restrict__ ids, int n, int64_t n_rows, int passes, uint32_t *__restrict__ key_out,
-                                                                uint32_t *__restrict__ pos_out, G *__restrict__ grad, int64_t zero_rows, int64_t width, int64_t ld)
+template <class G, bool NT>
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_one_tile(Ids ids, int n, int64_t n_rows, int passes, uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out,
+                                                                Zeros<G> z)
 {
     constexpr int ROUNDS = (int)(ONE_TILE / SORT_THREADS);
     __shared__ uint32_t at[SORT_WAVES][DIGITS], waves[SORT_WAVES], lkey[ONE_TILE];
     __shared__ uint16_t lpos[ONE_TILE];
     if (blockIdx.x > 0) {
-        fill_zero(grad, zero_rows, width, ld, blockIdx.x - 1, gridDim.x - 1);
+        fill_zero<G, NT>(z.grad, z.rows, z.width, z.ld, blockIdx.x - 1, gridDim.x - 1);
         return;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -309,32 +355,32 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_one_tile(const I *__restr
     }
 }
 
-// Sums. 2^lpr lanes take the columns of a tile (a lane one slot: a 16-byte chunk of grad_out's type, or one of the row's last elements),
-// and a group of lanes adds up the rows of SEG sorted entries. Ids that begin and end inside a group's entries are written at once;
-// the others meet in LDS, where the group in which an id begins adds what the following ones have of it; ids that cross the borders of a
-// workgroup's entries leave a sum before (part[0]) and behind (part[1]) the border for k_piece_join. Always ascending: the same bits.
+// Sums. 2^lpr lanes take the slots of a tile of columns, a group of lanes adds up the rows of SEG sorted entries. Ids that begin and end inside a
+// group's entries are written at once; of the others a group leaves in LDS what it has of an id that began before it (its head, `through` where
+// that goes on behind it) and of one that begins in it and goes on (its tail). Suffix sums over the heads, doubling their reach, give every
+// tail the rest of its id; ids that cross the borders of a workgroup's entries leave a sum before (part[0]) and behind (part[1]) the border
+// for k_piece_join. The order of the additions depends on n and width only.
 constexpr int SEG = 16;
 
-template <class G, int E> __device__ __forceinline__ void put_sum(G *p, const float (&sum)[E], int count, float scale, bool add)
+template <class T, class G, bool NT, bool NARROW> __device__ __forceinline__ void put_slot(G *row, const Slot<T> &at, const float (&sum)[Chunk<T>::N], float scale, bool add)
 {
+    constexpr int E = Chunk<T>::N, EG = Chunk<G>::N;         // E elements of grad_out's type are one or two chunks of grad's
+    if (NARROW || !at.whole()) {
 #pragma unroll
-    for (int i = 0; i < E; i++)
-        if (i < count) {
-            const float x = sum[i] * scale;
-            p[i] = from_float<G>(add ? to_float(p[i]) + x : x);
-        }
-}
-template <class G, int E> __device__ __forceinline__ void put_slot(G *p, const float (&sum)[E], bool vec, float scale, bool add)
-{
-    if (!vec) { put_sum<G, E>(p, sum, 1, scale, add); return; }
-    constexpr int EG = Chunk<G>::N;          // E of grad_out's type are one or two chunks of grad's
+        for (int i = 0; i < E; i++)
+            if (i >= at.skip && i < at.skip + at.count) {
+                const float x = sum[i] * scale;
+                row[at.j + i] = from_float<G>(add ? to_float(row[at.j + i]) + x : x);
+            }
+        return;
+    }
 #pragma unroll
     for (int c = 0; c < E / EG; c++) {
         float f[EG] = {};
-        if (add) load_chunk(p + c * EG, f);
+        if (add) load_chunk<false>(row + at.j + c * EG, f);
 #pragma unroll
         for (int i = 0; i < EG; i++) f[i] = add ? f[i] + sum[c * EG + i] * scale : sum[c * EG + i] * scale;
-        store_chunk(p + c * EG, f);
+        store_chunk<NT>(row + at.j + c * EG, f);
     }
 }
 
@@ -346,99 +392,121 @@ struct SumArgs {
     float *part;                             // [pieces][2][slots][E]
 };
 
-template <class T, class G>
+template <class T, class G, bool NT, bool NARROW>
 __global__ __launch_bounds__(256) void k_piece_sums(const T *__restrict__ gout, G *__restrict__ grad, SumArgs a)
 {
-    constexpr int E = Chunk<T>::N;
-    __shared__ float head[256][E], tail[256][E];
-    __shared__ uint8_t kind[256];            // per group: 1 its first id began before it, 2 that id goes on behind it, 4 its last id begins here and goes on
-    const int lane = threadIdx.x & ((1 << a.lpr) - 1), group = threadIdx.x >> a.lpr, groups = 256 >> a.lpr;
-    const int64_t per = (int64_t)groups * SEG;
+    constexpr int E = Chunk<T>::N, STEP = 4;
+    extern __shared__ uint32_t keys[];                                   // the workgroup's entries, the one before them and the one behind; then their places
+    __shared__ float head[256][E];
+    __shared__ uint8_t through[256];
+    const int lane = threadIdx.x & ((1 << a.lpr) - 1), group = threadIdx.x >> a.lpr, groups = 256 >> a.lpr, per = groups * SEG;
+    uint32_t *places = keys + per + 2;
+    const uint32_t none = 0xffffffffu;                                   // a key that no entry has
     for (int64_t b = blockIdx.x; b < a.pieces * a.tiles; b += gridDim.x) {
-        const int64_t piece = b / a.tiles, slot = ((b % a.tiles) << a.lpr) + lane;
-        const int64_t lo = piece * per + group * SEG;
-        const int64_t chunks = a.width / E;
-        const bool vec = slot < chunks, mine = slot < a.slots;
-        const int64_t j = vec ? slot * E : chunks * E + (slot - chunks);
-        uint32_t k[SEG], p[SEG];
+        const int64_t piece = b / a.tiles, slot = ((b % a.tiles) << a.lpr) + lane, lo = piece * per;
+        for (int i = threadIdx.x; i < per; i += 256) {
+            keys[i + 1] = lo + i < a.n ? a.key[lo + i] : none;
+            places[i] = lo + i < a.n ? a.pos[lo + i] : 0;
+        }
+        if (threadIdx.x == 0) keys[0] = lo > 0 ? a.key[lo - 1] : none;
+        if (threadIdx.x == 64) keys[per + 1] = lo + per < a.n ? a.key[lo + per] : none;
+        __syncthreads();
+        const uint32_t *k = keys + 1 + group * SEG, *p = places + group * SEG;
+        const bool mine = slot < a.slots;
+        const Slot<T> at(mine ? slot : 0, a.width);
+        u32x4 raw[SEG];
 #pragma unroll
         for (int i = 0; i < SEG; i++) {
-            const bool in = lo + i < a.n;
-            k[i] = in ? a.key[lo + i] : (uint32_t)a.n_rows;
-            p[i] = in ? a.pos[lo + i] : 0;
+            // (absent entries' rows are loaded too where a group has others: one wait for all, and their values are not looked at)
+            const T *row = gout + (int64_t)p[i] * a.ldg + at.j;
+            if constexpr (NARROW) {
+                union { u32x4 v; T e[E]; } u;
+                u.v = u32x4(0);
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (e < at.count) u.e[e] = row[e];
+                raw[i] = u.v;
+            } else raw[i] = load_raw<NT>(row);
         }
-        const uint32_t before = lo > 0 && lo < a.n ? a.key[lo - 1] : 0xffffffffu, after = lo + SEG < a.n ? a.key[lo + SEG] : 0xffffffffu;
-        int what = 0;
-        uint32_t last = 0;
-        float sum[E] = {};
-        bool first = true;
+        float sum[E] = {};                                               // (in the end the tail, where one begins)
+        bool first = true, goes_on = false, begins = false, began = false;
+        uint32_t last = none;
+        // (rolled, the registers moving along: the code that writes a finished sum is there STEP times instead of SEG)
+#pragma unroll 1
+        for (int i0 = 0; i0 < SEG; i0 += STEP) {
 #pragma unroll
-        for (int i0 = 0; i0 < SEG; i0 += 8) {
-            float f[8][E];
+            for (int i = 0; i < STEP; i++) {
+                const uint32_t key = k[i0 + i], next = k[i0 + i + 1];
+                if (key < (uint32_t)a.n_rows) {                          // absent entries are behind all others
+                    float f[E];
+                    unpack<T>(raw[i], f);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+                    for (int e = 0; e < E; e++) sum[e] += f[e];
+                    const bool end = i0 + i == SEG - 1;
+                    if (end || next != key) {
+                        if (first && k[-1] == key) {
+                            began = true;
+                            goes_on = end && next == key;
 #pragma unroll
-                for (int e = 0; e < E; e++) f[i][e] = 0.0f;
-                if (mine && k[i0 + i] < (uint32_t)a.n_rows) {
-                    const T *row = gout + (int64_t)p[i0 + i] * a.ldg + j;
-                    if (vec) load_chunk(row, f[i]);
-                    else f[i][0] = to_float(row[0]);
+                            for (int e = 0; e < E; e++) head[threadIdx.x][e] = sum[e];
+                        } else if (end && next == key) {
+                            begins = true;
+                            last = key;
+                        } else if (mine) put_slot<T, G, NT, NARROW>(grad + (int64_t)key * a.ld, at, sum, a.scale, a.add);
+#pragma unroll
+                        for (int e = 0; e < E; e++) sum[e] = begins ? sum[e] : 0.0f;
+                        first = false;
+                    }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint32_t key = k[i0 + i];
-                if (key >= (uint32_t)a.n_rows) continue;             // absent entries, and those behind the list, are last
+            for (int i = 0; i + STEP < SEG; i++) raw[i] = raw[i + STEP];
+        }
+        if (lane == 0) through[group] = goes_on;
+        if (__syncthreads_or(goes_on)) {
+            for (int reach = 1; reach < groups; reach <<= 1) {
+                const bool more = through[group] && group + reach < groups;
+                float rest[E] = {};
+                bool on = through[group];
+                if (more) {
 #pragma unroll
-                for (int e = 0; e < E; e++) sum[e] += f[i][e];
-                const bool end = i0 + i == SEG - 1;
-                const uint32_t next = end ? after : k[(i0 + i + 1) & (SEG - 1)];
-                if (!end && next == key) continue;
-                if (first && before == key) {
-                    what |= end && next == key ? 3 : 1;
+                    for (int e = 0; e < E; e++) rest[e] = head[threadIdx.x + (reach << a.lpr)][e];
+                    on = through[group + reach];
+                }
+                __syncthreads();
+                if (more) {
 #pragma unroll
-                    for (int e = 0; e < E; e++) head[threadIdx.x][e] = sum[e];
-                } else if (end && next == key) {
-                    what |= 4;
-                    last = key;
-#pragma unroll
-                    for (int e = 0; e < E; e++) tail[threadIdx.x][e] = sum[e];
-                } else if (mine) put_slot<G, E>(grad + (int64_t)key * a.ld + j, sum, vec, a.scale, a.add);
-#pragma unroll
-                for (int e = 0; e < E; e++) sum[e] = 0.0f;
-                first = false;
+                    for (int e = 0; e < E; e++) head[threadIdx.x][e] += rest[e];
+                    if (lane == 0) through[group] = on;
+                }
+                __syncthreads();
             }
         }
-        if (lane == 0) kind[group] = (uint8_t)what;
-        __syncthreads();
-        // an id that begins in this group (its tail), and in group 0 also the one that began before the workgroup's entries
-        for (int side = group == 0 ? 0 : 1; side < 2; side++) {
-            if (side == 0 ? !(what & 1) : !(what & 4)) continue;
-            int q = side == 0 ? 0 : group + 1;
-            bool on = side == 0 ? (what & 2) : true;                 // goes on behind group q (side 0) or into it (side 1)
+        // heads hold the rest of their id in this workgroup now, `through` whether it goes on behind the workgroup's entries
+        if (mine && group == 0 && began) {
+            float *out = a.part + (piece * 2 * a.slots + slot) * E;
 #pragma unroll
-            for (int e = 0; e < E; e++) sum[e] = side == 0 ? head[threadIdx.x][e] : tail[threadIdx.x][e];
-            if (side == 0) q = 1;
-            while (on && q < groups) {
+            for (int e = 0; e < E; e++) out[e] = head[threadIdx.x][e];
+        }
+        if (mine && begins) {
+            const bool here = group + 1 < groups;
+            if (here)
 #pragma unroll
-                for (int e = 0; e < E; e++) sum[e] += head[(q << a.lpr) + lane][e];
-                on = kind[q] & 2;
-                q++;
-            }
-            if (!mine) continue;
-            if (side == 0 || on) {
-                float *out = a.part + ((piece * 2 + side) * a.slots + slot) * E;
+                for (int e = 0; e < E; e++) sum[e] += head[threadIdx.x + (1 << a.lpr)][e];
+            if (here && !through[group + 1]) put_slot<T, G, NT, NARROW>(grad + (int64_t)last * a.ld, at, sum, a.scale, a.add);
+            else {
+                float *out = a.part + ((piece * 2 + 1) * a.slots + slot) * E;
 #pragma unroll
                 for (int e = 0; e < E; e++) out[e] = sum[e];
-            } else put_slot<G, E>(grad + (int64_t)last * a.ld + j, sum, vec, a.scale, a.add);
+            }
         }
         __syncthreads();
     }
 }
 
-// Ids that cross the border of two pieces: the workgroup of the piece in which one begins adds its sums in the order of the pieces,
-// its groups of lanes consecutive parts of them.
-template <class T, class G>
+// Ids that cross the border of two pieces: the workgroup of the piece in which one begins adds the sums of its pieces, every group of lanes
+// each groups-th of them, then the groups' sums by halves.
+template <class T, class G, bool NT, bool NARROW>
 __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArgs a)
 {
     constexpr int E = Chunk<T>::N;
@@ -447,124 +515,245 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
     const int64_t per = (int64_t)groups * SEG;
     for (int64_t b = blockIdx.x; b < (a.pieces - 1) * a.tiles; b += gridDim.x) {
         const int64_t piece = b / a.tiles, slot = ((b % a.tiles) << a.lpr) + lane, lo = piece * per, hi = lo + per;       // hi < n
-        const uint32_t k = a.key[hi - 1];
-        if (k >= (uint32_t)a.n_rows || a.key[hi] != k || (piece && a.key[lo - 1] == k)) continue;
-        // the last piece whose first entry has this id
-        int64_t x = piece + 1, y = a.pieces;
-        while (y - x > 1) {
-            const int64_t m = (x + y) / 2;
-            if (a.key[m * per] == k) x = m;
-            else y = m;
+        const uint32_t k = a.key[hi - 1], before = piece ? a.key[lo - 1] : 0xffffffffu;
+        if (k >= (uint32_t)a.n_rows || before == k) continue;
+        // how many of the next pieces begin with this id: 64 are asked at a time
+        int64_t count = 0;
+        for (bool on = true; on;) {
+            const int64_t q = piece + 1 + count + (threadIdx.x & 63);
+            const uint64_t other = ~__ballot(q < a.pieces && a.key[q * per] == k);
+            on = other == 0;
+            count += on ? 64 : __ffsll((unsigned long long)other) - 1;
         }
-        const int64_t count = x - piece, share = (count + groups - 1) / groups;          // sums of pieces piece + 1 .. x, and the tail of `piece`
-        const int64_t from = piece + 1 + group * share, to = from + share < x + 1 ? from + share : x + 1;
+        if (count == 0) continue;
         const bool mine = slot < a.slots;
         float sum[E] = {};
         if (mine) {
-            if (group == 0)
-#pragma unroll
-                for (int e = 0; e < E; e++) sum[e] = a.part[((piece * 2 + 1) * a.slots + slot) * E + e];
+            // pieces piece + 1 .. piece + count, and as number 0 the tail of `piece`
 #pragma unroll 4
-            for (int64_t q = from; q < to; q++)
+            for (int64_t q = group; q <= count; q += groups) {
+                const float *in = a.part + (((piece + q) * 2 + (q == 0)) * a.slots + slot) * E;
 #pragma unroll
-                for (int e = 0; e < E; e++) sum[e] += a.part[((q * 2) * a.slots + slot) * E + e];
+                for (int e = 0; e < E; e++) sum[e] += in[e];
+            }
         }
 #pragma unroll
         for (int e = 0; e < E; e++) sums[threadIdx.x][e] = sum[e];
         __syncthreads();
-        if (group == 0 && mine) {
-            for (int q = 1; q < groups; q++)
+        for (int half = groups >> 1; half; half >>= 1) {
+            if (group < half)
 #pragma unroll
-                for (int e = 0; e < E; e++) sum[e] += sums[(q << a.lpr) + lane][e];
-            const int64_t chunks = a.width / E;
-            const bool vec = slot < chunks;
-            put_slot<G, E>(grad + (int64_t)k * a.ld + (vec ? slot * E : chunks * E + (slot - chunks)), sum, vec, a.scale, a.add);
+                for (int e = 0; e < E; e++) sums[threadIdx.x][e] += sums[threadIdx.x + (half << a.lpr)][e];
+            __syncthreads();
+        }
+        if (group == 0 && mine) {
+#pragma unroll
+            for (int e = 0; e < E; e++) sum[e] = sums[threadIdx.x][e];
+            put_slot<T, G, NT, NARROW>(grad + (int64_t)k * a.ld, Slot<T>(slot, a.width), sum, a.scale, a.add);
         }
         __syncthreads();
     }
 }
 
 // ---------------------------------------------------------------------------------------------- log-likelihood of a token
-// running maximum and sum of a softmax: exp(x - m) is added to s, s is rescaled where the maximum grows. A maximum of -infinity
-// (nothing but excluded classes so far) counts as 0 in the differences, so that they stay -infinity and add 0.
+// Forward: one read of the row with the running maximum and sum of a softmax. A lane takes BATCH chunks at a time: their maximum first, one
+// rescaling of the sum, then the exponentials. A maximum of -infinity (nothing but excluded classes so far) counts as 0 in the differences,
+// so that they stay -infinity and add 0. LANES lanes take a row; few long rows are cut into parts whose (max, sum) a second launch joins.
+// exp(t) = 2^(t log2 e) with log2 e in two parts: one part alone is off by 1.3e-8 of t in every term alike, 1e-7 of a typical row's sum, and
+// a pair's margin adds that up over hundreds of tokens (measured: margins of 512-token pairs off by 4e-6, with both parts by 5e-7).
+constexpr float LOG2E_HI = LOG2E, LOG2E_LO = 1.92596299e-8f;       // log2 e = 1.44269502162933 + 1.92596299e-8
+constexpr int BATCH = 4;
+
 struct MaxSum { float m, s; };
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(__builtin_fmaf(t, LOG2E_HI, t * LOG2E_LO)); }       // (one rounding at the large part's size)
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));       // fmaxf would quiet both operands first, an operation each
+    return d;
+}
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b)
 {
     const float m = fmaxf(a.m, b.m), r = finite_max(m);
-    return { m, a.s * __builtin_amdgcn_exp2f((a.m - r) * LOG2E) + b.s * __builtin_amdgcn_exp2f((b.m - r) * LOG2E) };
+    return { m, a.s * exp_of(a.m - r) + b.s * exp_of(b.m - r) };
 }
-__device__ __forceinline__ void add_one(MaxSum &a, float x)
+template <int N> __device__ __forceinline__ void add_values(MaxSum &a, const float (&f)[N])
 {
-    const float m = fmaxf(a.m, x), r = finite_max(m);
-    a.s = a.s * __builtin_amdgcn_exp2f((a.m - r) * LOG2E) + __builtin_amdgcn_exp2f((x - r) * LOG2E);
-    a.m = m;
+    float m = a.m;
+    if constexpr (N % 2) m = fmaxf(m, f[N - 1]);
+#pragma unroll
+    for (int i = 0; i + 1 < N; i += 2) m = max3(m, f[i], f[i + 1]);
+    const float r = finite_max(m);
+    float s = a.s * exp_of(a.m - r);
+    float more[4] = {};
+#pragma unroll
+    for (int i = 0; i < N; i++) more[i & 3] += exp_of(f[i] - r);
+    a = { m, s + ((more[0] + more[1]) + (more[2] + more[3])) };
 }
-template <class T, class I>
-__global__ __launch_bounds__(256) void k_token_loglik(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, const I *__restrict__ target,
+template <class T> __device__ __forceinline__ uint32_t minus_infinities() { return sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, __bf16> ? 0xFF80FF80u : 0xFC00FC00u; }
+// Chunks c0 .. c1 of a row and its last elements (where `rest`) by LANES lanes. The next BATCH chunks are on their way while these are added:
+// two sets of registers, and loads that are always made (behind the end the last chunk again, its values left out), since a wait behind
+// loads that some lanes may have skipped is a wait for all of them.
+template <class T, bool NT, int LANES> __device__ __forceinline__ MaxSum row_part(const T *x, int64_t c0, int64_t c1, int64_t classes, bool rest, int lane)
+{
+    constexpr int E = Chunk<T>::N, STEP = BATCH * LANES;
+    MaxSum a = { -INFINITY, 0.0f };
+    typedef u32x4 Set[BATCH];
+    auto fetch = [&](Set &v, int64_t base) {
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) {
+            const int64_t c = base + i * LANES + lane;
+            v[i] = load_raw<NT>(x + (c < c1 ? c : c1 - 1) * E);
+        }
+    };
+    auto add = [&](Set &v, int64_t base) {
+        if (base + STEP > c1)
+#pragma unroll
+            for (int i = 0; i < BATCH; i++)
+                if (base + i * LANES + lane >= c1) v[i] = u32x4(minus_infinities<T>());
+        float f[BATCH * E];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) unpack<T>(v[i], f + i * E);
+        add_values(a, f);
+    };
+    if (c0 < c1) {
+        Set p, q;
+        fetch(p, c0);
+        for (int64_t base = c0;; base += 2 * STEP) {
+            if (base + STEP >= c1) { add(p, base); break; }
+            fetch(q, base + STEP);
+            __builtin_amdgcn_sched_barrier(0);
+            add(p, base);
+            if (base + 2 * STEP >= c1) { add(q, base + STEP); break; }
+            fetch(p, base + 2 * STEP);
+            __builtin_amdgcn_sched_barrier(0);
+            add(q, base + STEP);
+        }
+    }
+    const int64_t j = classes / E * E + lane;
+    if (rest && j < classes) {
+        const float f[1] = { to_float(x[j]) };
+        add_values(a, f);
+    }
+    return a;
+}
+template <int LANES> __device__ __forceinline__ MaxSum join_lanes(MaxSum a, MaxSum *ws)
+{
+#pragma unroll
+    for (int m = LANES < 64 ? LANES / 2 : 32; m; m >>= 1) a = join(a, { __shfl_xor(a.m, m), __shfl_xor(a.s, m) });
+    if constexpr (LANES > 64) {
+        if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = a;
+        __syncthreads();
+        a = ws[0];
+#pragma unroll
+        for (int w = 1; w < LANES / 64; w++) a = join(a, ws[w]);
+        __syncthreads();
+    }
+    return a;
+}
+// the last steps in 64 bits: a pair's margin adds up small differences of many of these
+__device__ __forceinline__ void put_loglik(float *logp, float *stats, int64_t t, MaxSum a, float value)
+{
+    const double log_sum = log((double)a.s);
+    logp[t] = a.m == -INFINITY && a.s == 0.0f ? -INFINITY : (float)(((double)value - (double)a.m) - log_sum);
+    stats[2 * t] = a.m;
+    stats[2 * t + 1] = (float)log_sum;
+}
+template <class T, bool NT, int LANES>
+__global__ __launch_bounds__(256) void k_token_loglik(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target,
                                                       float *__restrict__ logp, float *__restrict__ stats)
 {
-    constexpr int E = Chunk<T>::N;
+    constexpr int ROWS = 256 / LANES;
     __shared__ MaxSum ws[4];
-    const int64_t chunks = classes / E;
-    for (int64_t t = blockIdx.x; t < n; t += gridDim.x) {
+    const int lane = threadIdx.x & (LANES - 1);
+    for (int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; t < n; t += (int64_t)gridDim.x * ROWS) {
         const int64_t y = id_at(target, t, classes);
         if (y < 0) {
-            if (threadIdx.x == 0) { logp[t] = 0.0f; stats[2 * t] = 0.0f; stats[2 * t + 1] = 0.0f; }
+            if (lane == 0) { logp[t] = 0.0f; stats[2 * t] = 0.0f; stats[2 * t + 1] = 0.0f; }
             continue;
         }
         const T *x = logits + t * ld;
-        MaxSum a = { -INFINITY, 0.0f };
-        for (int64_t c = threadIdx.x; c < chunks; c += 256) {
-            float f[E];
-            load_chunk(x + c * E, f);
-#pragma unroll
-            for (int i = 0; i < E; i++) add_one(a, f[i]);
-        }
-        if (threadIdx.x < classes % E) add_one(a, to_float(x[chunks * E + threadIdx.x]));
-#pragma unroll
-        for (int m = 32; m; m >>= 1) a = join(a, { __shfl_xor(a.m, m), __shfl_xor(a.s, m) });
-        if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = a;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            a = join(join(ws[0], ws[1]), join(ws[2], ws[3]));
-            // the last steps in 64 bits: a pair's margin adds up small differences of many of these
-            const double log_sum = log((double)a.s);
-            logp[t] = a.m == -INFINITY && a.s == 0.0f ? -INFINITY : (float)(((double)to_float(x[y]) - (double)a.m) - log_sum);
-            stats[2 * t] = a.m;
-            stats[2 * t + 1] = (float)log_sum;
-        }
-        __syncthreads();
+        const MaxSum a = join_lanes<LANES>(row_part<T, NT, LANES>(x, 0, classes / Chunk<T>::N, classes, true, lane), ws);
+        if (lane == 0) put_loglik(logp, stats, t, a, to_float(x[y]));
     }
 }
-template <class T, class I>
-__global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, int64_t n, int64_t classes, int64_t ld, const I *__restrict__ target,
-                                                               const float *__restrict__ stats, const float *__restrict__ gl, T *out, int64_t ldo)
+// parts of rows, [n][parts] of workspace; parts <= 64
+template <class T, bool NT>
+__global__ __launch_bounds__(256) void k_token_loglik_parts(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target, int parts,
+                                                            MaxSum *__restrict__ out)
 {
-    constexpr int E = Chunk<T>::N;
-    const int64_t chunks = classes / E;
-    for (int64_t t = blockIdx.x; t < n; t += gridDim.x) {
+    __shared__ MaxSum ws[4];
+    const int64_t t = blockIdx.x / parts, part = blockIdx.x % parts;
+    if (id_at(target, t, classes) < 0) return;
+    const int64_t chunks = classes / Chunk<T>::N, step = (chunks + parts - 1) / parts, c0 = part * step < chunks ? part * step : chunks, c1 = c0 + step < chunks ? c0 + step : chunks;
+    const MaxSum a = join_lanes<256>(row_part<T, NT, 256>(logits + t * ld, c0, c1, classes, part == parts - 1, threadIdx.x), ws);
+    if (threadIdx.x == 0) out[blockIdx.x] = a;
+}
+template <class T>
+__global__ __launch_bounds__(64) void k_token_loglik_join(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target, int parts,
+                                                          const MaxSum *__restrict__ in, float *__restrict__ logp, float *__restrict__ stats)
+{
+    const int64_t t = blockIdx.x, y = id_at(target, t, classes);
+    if (y < 0) {
+        if (threadIdx.x == 0) { logp[t] = 0.0f; stats[2 * t] = 0.0f; stats[2 * t + 1] = 0.0f; }
+        return;
+    }
+    MaxSum a = { -INFINITY, 0.0f };
+    if ((int)threadIdx.x < parts) a = in[t * parts + threadIdx.x];
+    a = join_lanes<64>(a, nullptr);
+    if (threadIdx.x == 0) put_loglik(logp, stats, t, a, to_float(logits[t * ld + y]));
+}
+// Backward: one read and one write of the row; the target's class as -expm1(log p), since 1 - p would lose the digits of a p near 1.
+// A workgroup takes ROWS rows of LANES lanes, or a part of a row.
+template <class T, bool NT, int LANES>
+__global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, int64_t n, int64_t classes, int64_t ld, Ids target,
+                                                               const float *__restrict__ stats, const float *__restrict__ gl, T *out, int64_t ldo, int64_t parts)
+{
+    constexpr int E = Chunk<T>::N, ROWS = 256 / LANES;
+    const int lane = threadIdx.x & (LANES - 1);
+    const int64_t chunks = classes / E, step = (chunks + parts - 1) / parts;
+    for (int64_t b = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; b < n * parts; b += (int64_t)gridDim.x * ROWS) {
+        const int64_t t = b / parts, part = b % parts;
         const int64_t y = id_at(target, t, classes);
-        const float g = gl[t], m = stats[2 * t], ls = stats[2 * t + 1] * LOG2E;
+        const float g = gl[t], m = stats[2 * t], log_sum = stats[2 * t + 1], ls = log_sum * LOG2E;
         const bool none = y < 0 || g == 0.0f || m == -INFINITY;
         const T *x = logits + t * ld;
         T *o = out + t * ldo;
-        // [j == y] - p, the target's as -expm1(log p): 1 - p would lose the digits of a p near 1
-        auto value = [&](float v, int64_t j) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(v - m, LOG2E, -ls));
-            return j == y ? g * -expm1f((v - m) - stats[2 * t + 1]) : -(g * p);
-        };
-        for (int64_t c = threadIdx.x; c < chunks; c += 256) {
-            float f[E] = {};
-            if (!none) {
-                load_chunk(x + c * E, f);
+        const int64_t c1 = (part + 1) * step < chunks ? (part + 1) * step : chunks;
+        auto other = [&](float v) { return -(g * __builtin_amdgcn_exp2f(__builtin_fmaf(v - m, LOG2E, -ls))); };
+        auto hit = [&](float v) { return g * -expm1f((v - m) - log_sum); };
+        auto slot = [&](int64_t c, float (&f)[E]) {
+            float h = 0.0f;
+            const bool here = c == y / E;
+            if (here) h = hit(to_float(x[y]));
 #pragma unroll
-                for (int i = 0; i < E; i++) f[i] = value(f[i], c * E + i);
+            for (int i = 0; i < E; i++) f[i] = other(f[i]);
+            if (here)
+#pragma unroll
+                for (int i = 0; i < E; i++) f[i] = i == (int)(y % E) ? h : f[i];
+            store_chunk<NT>(o + c * E, f);
+        };
+        int64_t c = part * step + lane;
+        if (none) {
+            const float zero[E] = {};
+            for (; c < c1; c += LANES) store_chunk<NT>(o + c * E, zero);
+        } else {
+            for (; c + (BATCH - 1) * LANES < c1; c += BATCH * LANES) {
+                float f[BATCH][E];
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) load_chunk<NT>(x + (c + i * LANES) * E, f[i]);
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) slot(c + i * LANES, f[i]);
             }
-            store_chunk(o + c * E, f);
+            for (; c < c1; c += LANES) {
+                float f[E];
+                load_chunk<NT>(x + c * E, f);
+                slot(c, f);
+            }
         }
-        const int64_t j = chunks * E + threadIdx.x;
-        if (j < classes) o[j] = from_float<T>(none ? 0.0f : value(to_float(x[j]), j));
+        const int64_t j = chunks * E + lane;
+        if (part == parts - 1 && j < classes) o[j] = from_float<T>(none ? 0.0f : j == y ? hit(to_float(x[j])) : other(to_float(x[j])));
     }
 }
 
@@ -696,7 +885,7 @@ template <class F> int by_type(int32_t type, F &&f)
 {
     return type == MLX_F32 ? f(float()) : type == MLX_BF16 ? f(__bf16()) : f(_Float16());
 }
-template <class F> int by_id(int32_t id_type, F &&f) { return id_type == MLX_I32 ? f(int32_t()) : f(int64_t()); }
+template <class F> int by_flag(bool flag, F &&f) { return flag ? f(std::true_type()) : f(std::false_type()); }
 
 int check_matrix(const char *who, const char *what, const void *p, int64_t rows, int64_t width, int64_t ld, int64_t es, bool output)
 {
@@ -707,6 +896,10 @@ int check_matrix(const char *who, const char *what, const void *p, int64_t rows,
     return MLX_OK;
 }
 
+// Matrices that are read or written once and do not fit the caches go past their usual replacement (non-temporal).
+constexpr int64_t CACHED = 32 << 20;
+bool streams(int64_t rows, int64_t width, int64_t es) { return rows * width * es > CACHED; }
+
 struct GradientPlan { SortPlan sort; int lpr; int64_t slots, tiles, pieces; size_t key, counts, part, bytes; };
 GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
 {
@@ -716,17 +909,34 @@ GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
     g.sort.tiles = (int)ceil_div(n, g.sort.tile);
     g.sort.passes = 1;
     while (n_rows >> (g.sort.passes * DIGIT_BITS)) g.sort.passes++;          // keys run from 0 to n_rows
-    g.slots = width / E + width % E;
+    g.slots = slots_of(width, E);
     g.lpr = 0;
     while (g.lpr < 6 && (1 << g.lpr) < g.slots) g.lpr++;
     g.tiles = ceil_div(g.slots, 1 << g.lpr);
     g.pieces = ceil_div(n, (int64_t)(256 >> g.lpr) * SEG);
     auto round = [](size_t b) { return (b + 255) / 256 * 256; };
     g.key = round((size_t)n * 4);
-    g.counts = n <= ONE_TILE ? 0 : round((size_t)g.sort.passes * g.sort.tiles * DIGITS * 4);
+    g.counts = n <= ONE_TILE ? 0 : round((size_t)g.sort.tiles * DIGITS * 4);
     g.part = g.pieces > 1 ? round((size_t)g.pieces * 2 * (size_t)g.slots * (size_t)E * 4) : 0;
     g.bytes = 4 * g.key + g.counts + g.part;
     return g;
+}
+
+// Lanes of a row: enough that a lane has a few chunks, 8 at least. Rows are cut into parts where they are too few to fill the chip:
+// parts of 4 chunks a lane or more, 64 at most (the lanes of the wave that joins them), 512 workgroups in all.
+struct LoglikPlan { int lanes, parts; size_t bytes; };
+LoglikPlan loglik_plan(int64_t es, int64_t n, int64_t classes)
+{
+    LoglikPlan p;
+    const int64_t chunks = classes * es / 16;
+    p.lanes = chunks <= 8 * BATCH ? 8 : chunks <= 64 * BATCH ? 64 : 256;
+    p.parts = n >= 512 || n == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({ 64, ceil_div(512, n), chunks / (256 * BATCH) }));
+    p.bytes = p.parts > 1 ? (size_t)(n * p.parts) * sizeof(MaxSum) : 0;
+    return p;
+}
+template <class F> int by_lanes(int lanes, F &&f)
+{
+    return lanes == 8 ? f(std::integral_constant<int, 8>()) : lanes == 64 ? f(std::integral_constant<int, 64>()) : f(std::integral_constant<int, 256>());
 }
 
 }  // namespace
@@ -752,15 +962,16 @@ int mlx_embedding_lookup(int32_t device, void *stream, int32_t type, const void 
     if (on.rc) return on.rc;
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
-        return by_id(id_type, [&](auto i) {
-            typedef decltype(i) I;
-            const int64_t slots = width / Chunk<T>::N + width % Chunk<T>::N;
-            int lpr = 0;
-            while (lpr < 8 && (1 << lpr) < slots) lpr++;
-            const int64_t groups = ceil_div(n_ids, 256 >> lpr);
-            hipLaunchKernelGGL((k_embedding_lookup<T, I>), dim3(grid_of(groups)), dim3(256), 0, (hipStream_t)stream, (const T *)table, n_rows, width, ld_table,
-                               (const I *)ids, n_ids, scale, (T *)out, ld_out, lpr, groups);
-            return 0;
+        return by_flag(streams(n_ids, width, es), [&](auto nt) {
+            return by_flag(width < Chunk<T>::N, [&](auto narrow) {
+                const int64_t slots = slots_of(width, Chunk<T>::N);
+                int lpr = 0;
+                while (lpr < 8 && (1 << lpr) < slots) lpr++;
+                const int64_t groups = ceil_div(n_ids, 256 >> lpr);
+                hipLaunchKernelGGL((k_embedding_lookup<T, nt.value, narrow.value>), dim3(grid_of(groups)), dim3(256), 0, (hipStream_t)stream, (const T *)table, n_rows, width,
+                                   ld_table, Ids{ ids, id_type == MLX_I64 }, n_ids, scale, (T *)out, ld_out, lpr, groups);
+                return 0;
+            });
         });
     });
     return launched(who);
@@ -802,52 +1013,55 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
     uint32_t *key[2] = { (uint32_t *)w, (uint32_t *)(w + plan.key) }, *pos[2] = { (uint32_t *)(w + 2 * plan.key), (uint32_t *)(w + 3 * plan.key) };
     uint32_t *counts = (uint32_t *)(w + 4 * plan.key);
     float *part = (float *)(w + 4 * plan.key + plan.counts);
-    auto with = [&](auto t, auto g) {
+    auto with = [&](auto t, auto g, auto nt, auto narrow) {
         typedef decltype(t) T;
         typedef decltype(g) G;
-        return by_id(id_type, [&](auto i) {
-            typedef decltype(i) I;
-            const I *id = (const I *)ids;
-            G *out = (G *)grad;
-            // The zeros of grad go along with the sort's launches, each a share of the rows: the few workgroups of the sort run beside them.
-            const int shares = n_ids <= ONE_TILE ? 1 : plan.sort.passes + 1;
-            int64_t row = 0;
-            struct Share { G *at; int64_t rows; unsigned blocks; };
-            auto zeros = [&](int k) {
-                const int64_t end = accumulate ? 0 : n_rows * (k + 1) / shares, rows = end - row;
-                Share s = { out + row * ld_grad, rows, 0 };
-                if (rows > 0) s.blocks = (unsigned)std::min<int64_t>(2048, ceil_div(rows * width, 4 * SORT_THREADS * Chunk<G>::N));
-                row = end;
-                return s;
-            };
-            int cur = 0;
-            if (n_ids <= ONE_TILE) {
-                const Share z = zeros(0);
-                hipLaunchKernelGGL((k_sort_one_tile<G, I>), dim3(1 + z.blocks), dim3(SORT_THREADS), 0, st, id, (int)n_ids, n_rows, plan.sort.passes, key[0], pos[0], z.at, z.rows,
-                                   width, ld_grad);
-            } else {
-                Share z = zeros(0);
-                hipLaunchKernelGGL((k_sort_begin<G, I>), dim3(plan.sort.tiles + z.blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, counts, z.at, z.rows, width,
-                                   ld_grad);
-                for (int pass = 0; pass < plan.sort.passes; pass++) {
-                    z = zeros(pass + 1);
-                    if (pass == 0)
-                        hipLaunchKernelGGL((k_sort_pass<G, I, true>), dim3(plan.sort.tiles + z.blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, pass, counts,
-                                           nullptr, nullptr, key[0], pos[0], z.at, z.rows, width, ld_grad);
-                    else
-                        hipLaunchKernelGGL((k_sort_pass<G, I, false>), dim3(plan.sort.tiles + z.blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, pass, counts,
-                                           key[cur], pos[cur], key[cur ^ 1], pos[cur ^ 1], z.at, z.rows, width, ld_grad);
-                    if (pass) cur ^= 1;
-                }
-            }
-            if (n_ids == 0) return 0;
-            const SumArgs a = { key[cur], pos[cur], n_ids, n_rows, width, ld_grad_out, ld_grad, plan.slots, plan.tiles, plan.pieces, scale, accumulate != 0, plan.lpr, part };
-            hipLaunchKernelGGL((k_piece_sums<T, G>), dim3(grid_of(plan.pieces * plan.tiles)), dim3(256), 0, st, (const T *)grad_out, out, a);
-            if (plan.pieces > 1) hipLaunchKernelGGL((k_piece_join<T, G>), dim3(grid_of((plan.pieces - 1) * plan.tiles)), dim3(256), 0, st, out, a);
-            return 0;
-        });
+        constexpr bool NT = decltype(nt)::value, NARROW = decltype(narrow)::value;
+        const Ids id = { ids, id_type == MLX_I64 };
+        G *out = (G *)grad;
+        // The zeros of grad go along with the sort's launches, each a share of the rows: the few workgroups of the sort run beside them.
+        const int shares = n_ids <= ONE_TILE ? 1 : 2 * plan.sort.passes;
+        int64_t row = 0;
+        int share = 0;
+        unsigned blocks = 0;
+        auto zeros = [&]() {
+            const int64_t end = accumulate ? 0 : n_rows * ++share / shares, rows = end - row;
+            const Zeros<G> z = { out + row * ld_grad, rows, width, ld_grad };
+            blocks = rows > 0 ? (unsigned)std::min<int64_t>(2048, ceil_div(rows * width, 4 * SORT_THREADS * Chunk<G>::N)) : 0;
+            row = end;
+            return z;
+        };
+        int cur = 0;
+        if (n_ids <= ONE_TILE) {
+            const Zeros<G> z = zeros();
+            hipLaunchKernelGGL((k_sort_one_tile<G, NT>), dim3(1 + blocks), dim3(SORT_THREADS), 0, st, id, (int)n_ids, n_rows, plan.sort.passes, key[0], pos[0], z);
+        } else
+            for (int pass = 0; pass < plan.sort.passes; pass++)
+                by_flag(pass == 0, [&](auto first) {
+                    constexpr bool FIRST = decltype(first)::value;
+                    const int shift = pass * DIGIT_BITS;
+                    Zeros<G> z = zeros();
+                    hipLaunchKernelGGL((k_sort_count<G, NT, FIRST>), dim3(plan.sort.tiles + blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, shift, counts,
+                                       key[cur], z);
+                    z = zeros();
+                    const int to = FIRST ? 0 : cur ^ 1;
+                    hipLaunchKernelGGL((k_sort_move<G, NT, FIRST>), dim3(plan.sort.tiles + blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, shift, counts,
+                                       key[cur], pos[cur], key[to], pos[to], z);
+                    cur = to;
+                    return 0;
+                });
+        if (n_ids == 0) return 0;
+        const SumArgs a = { key[cur], pos[cur], n_ids, n_rows, width, ld_grad_out, ld_grad, plan.slots, plan.tiles, plan.pieces, scale, accumulate != 0, plan.lpr, part };
+        hipLaunchKernelGGL((k_piece_sums<T, G, NT, NARROW>), dim3(grid_of(plan.pieces * plan.tiles)), dim3(256), (2 * (256 >> plan.lpr) * SEG + 2) * sizeof(uint32_t),
+                           st, (const T *)grad_out, out, a);
+        if (plan.pieces > 1) hipLaunchKernelGGL((k_piece_join<T, G, NT, NARROW>), dim3(grid_of((plan.pieces - 1) * plan.tiles)), dim3(256), 0, st, out, a);
+        return 0;
     };
-    by_type(type, [&](auto t) { return grad_type == MLX_F32 ? with(t, float()) : with(t, t); });
+    by_type(type, [&](auto t) {
+        return by_flag(streams(n_rows, width, gs), [&](auto nt) {
+            return by_flag(width < Chunk<decltype(t)>::N, [&](auto narrow) { return grad_type == MLX_F32 ? with(t, float(), nt, narrow) : with(t, t, nt, narrow); });
+        });
+    });
     return launched(who);
 }
 
@@ -856,7 +1070,7 @@ int mlx_token_loglik_workspace(int64_t n_tokens, int64_t n_classes, size_t *byte
     const char *who = "mlx_token_loglik_workspace";
     MLX_REFUSE(!bytes, "%s: bytes is NULL", who);
     MLX_REFUSE(n_tokens < 0 || n_tokens > MOST || n_classes < 1 || n_classes > MOST, "%s: bad sizes", who);
-    *bytes = 0;
+    *bytes = std::max(loglik_plan(4, n_tokens, n_classes).bytes, loglik_plan(2, n_tokens, n_classes).bytes);
     return MLX_OK;
 }
 
@@ -871,8 +1085,8 @@ int mlx_token_loglik(int32_t device, void *stream, int32_t type, const void *log
     if (n_tokens == 0) return MLX_OK;
     MLX_REFUSE(!target || (uintptr_t)target % (uintptr_t)is, "%s: target is NULL or not aligned", who);
     MLX_REFUSE(!logp || !stats || ((uintptr_t)logp | (uintptr_t)stats) % 4, "%s: logp or stats is NULL or not aligned", who);
-    size_t need;
-    if (int rc = mlx_token_loglik_workspace(n_tokens, n_classes, &need)) return rc;
+    const LoglikPlan plan = loglik_plan(es, n_tokens, n_classes);
+    const size_t need = plan.bytes;
     MLX_REFUSE(workspace_bytes < need, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, need);
     MLX_REFUSE(need && (!workspace || (uintptr_t)workspace % 256), "%s: workspace is NULL or not aligned to 256 bytes", who);
     const int64_t lb = span(n_tokens, n_classes, ld_logits, es);
@@ -882,10 +1096,23 @@ int mlx_token_loglik(int32_t device, void *stream, int32_t type, const void *log
     if (on.rc) return on.rc;
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
-        return by_id(id_type, [&](auto i) {
-            typedef decltype(i) I;
-            hipLaunchKernelGGL((k_token_loglik<T, I>), dim3(grid_of(n_tokens)), dim3(256), 0, (hipStream_t)stream, (const T *)logits, n_tokens, n_classes, ld_logits,
-                               (const I *)target, logp, stats);
+        return by_flag(streams(n_tokens, n_classes, es), [&](auto nt) {
+            constexpr bool NT = decltype(nt)::value;
+            hipStream_t st = (hipStream_t)stream;
+            const T *x = (const T *)logits;
+            const Ids y = { target, id_type == MLX_I64 };
+            if (plan.parts > 1) {
+                hipLaunchKernelGGL((k_token_loglik_parts<T, NT>), dim3((unsigned)(n_tokens * plan.parts)), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
+                                   (MaxSum *)workspace);
+                hipLaunchKernelGGL((k_token_loglik_join<T>), dim3((unsigned)n_tokens), dim3(64), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
+                                   (const MaxSum *)workspace, logp, stats);
+            } else
+                by_lanes(plan.lanes, [&](auto l) {
+                    constexpr int LANES = decltype(l)::value;
+                    hipLaunchKernelGGL((k_token_loglik<T, NT, LANES>), dim3(grid_of(ceil_div(n_tokens, 256 / LANES))), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, logp,
+                                       stats);
+                    return 0;
+                });
             return 0;
         });
     });
@@ -914,11 +1141,15 @@ int mlx_token_loglik_gradient(int32_t device, void *stream, int32_t type, const 
     if (on.rc) return on.rc;
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
-        return by_id(id_type, [&](auto i) {
-            typedef decltype(i) I;
-            hipLaunchKernelGGL((k_token_loglik_gradient<T, I>), dim3(grid_of(n_tokens)), dim3(256), 0, (hipStream_t)stream, (const T *)logits, n_tokens, n_classes,
-                               ld_logits, (const I *)target, stats, grad_logp, (T *)dlogits, ld_dlogits);
-            return 0;
+        return by_flag(streams(n_tokens, n_classes, es), [&](auto nt) {
+            const LoglikPlan plan = loglik_plan(es, n_tokens, n_classes);
+            return by_lanes(plan.lanes, [&](auto l) {
+                constexpr int LANES = decltype(l)::value;
+                hipLaunchKernelGGL((k_token_loglik_gradient<T, nt.value, LANES>), dim3(grid_of(ceil_div(n_tokens * plan.parts, 256 / LANES))), dim3(256), 0, (hipStream_t)stream,
+                                   (const T *)logits, n_tokens, n_classes, ld_logits, Ids{ target, id_type == MLX_I64 }, stats, grad_logp, (T *)dlogits, ld_dlogits,
+                                   (int64_t)plan.parts);
+                return 0;
+            });
         });
     });
     return launched(who);
