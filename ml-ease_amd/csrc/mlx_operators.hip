@@ -228,6 +228,18 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_move(Ids ids, int64_t n, 
         return;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t part = plan.tile / SORT_WAVES, end = (int64_t)(blockIdx.x + 1) * plan.tile < n ? (int64_t)(blockIdx.x + 1) * plan.tile : n;
+    const int64_t lo = (int64_t)blockIdx.x * plan.tile + wave * part, hi = lo + part < end ? lo + part : end;
+    uint32_t k[AHEAD], p[AHEAD];
+    auto fetch = [&](int64_t r) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int64_t i = r + a * 64 + lane, c = i < hi ? i : hi - 1;
+            k[a] = FIRST ? key_at(ids, c, n_rows) : key[c];
+            p[a] = FIRST ? (uint32_t)c : pos[c];
+        }
+    };
+    if (lo < hi) fetch(lo);
 #pragma unroll
     for (int w = 0; w < SORT_WAVES; w++) at[w][threadIdx.x] = 0;
     // this thread's digit: entries of it in the tiles before, and in all; COLUMN loads at a time (the last tile again behind the end)
@@ -243,19 +255,9 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_move(Ids ids, int64_t n, 
         }
     }
     const uint32_t first = digits_before(all, waves) + before;       // (synchronises: `at` is zero behind it)
-    const int64_t part = plan.tile / SORT_WAVES, end = (int64_t)(blockIdx.x + 1) * plan.tile < n ? (int64_t)(blockIdx.x + 1) * plan.tile : n;
-    const int64_t lo = (int64_t)blockIdx.x * plan.tile + wave * part, hi = lo + part < end ? lo + part : end;
-    uint32_t k[AHEAD], p[AHEAD];
-    auto fetch = [&](int64_t r, bool places) {
-#pragma unroll
-        for (int a = 0; a < AHEAD; a++) {
-            const int64_t i = r + a * 64 + lane, c = i < hi ? i : hi - 1;
-            k[a] = FIRST ? key_at(ids, c, n_rows) : key[c];
-            if (places) p[a] = FIRST ? (uint32_t)c : pos[c];
-        }
-    };
+    const bool more = part > AHEAD * 64;                             // a wave's part is more than the registers hold: read again
     for (int64_t r = lo; r < hi; r += AHEAD * 64) {
-        fetch(r, false);
+        if (r > lo) fetch(r);
 #pragma unroll
         for (int a = 0; a < AHEAD; a++)
             if (r + a * 64 + lane < hi) atomicAdd(&at[wave][(k[a] >> shift) & (DIGITS - 1)], 1u);
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_move(Ids ids, int64_t n, 
     }
     __syncthreads();
     for (int64_t r = lo; r < hi; r += AHEAD * 64) {
-        fetch(r, true);
+        if (more) fetch(r);
 #pragma unroll
         for (int a = 0; a < AHEAD; a++) {
             const bool here = r + a * 64 + lane < hi;
@@ -360,7 +362,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_one_tile(Ids ids, int n, 
 // that goes on behind it) and of one that begins in it and goes on (its tail). Suffix sums over the heads, doubling their reach, give every
 // tail the rest of its id; ids that cross the borders of a workgroup's entries leave a sum before (part[0]) and behind (part[1]) the border
 // for k_piece_join. The order of the additions depends on n and width only.
-constexpr int SEG = 16;
+constexpr int SEG = 8;
 
 template <class T, class G, bool NT, bool NARROW> __device__ __forceinline__ void put_slot(G *row, const Slot<T> &at, const float (&sum)[Chunk<T>::N], float scale, bool add)
 {
@@ -392,11 +394,12 @@ struct SumArgs {
     float *part;                             // [pieces][2][slots][E]
 };
 
-template <class T, class G, bool NT, bool NARROW>
+// WAVE: a group is a wave (lpr == 6): keys and places are a lane's each, read from there into scalar registers, and the branches are the wave's.
+template <class T, class G, bool NT, bool NARROW, bool WAVE>
 __global__ __launch_bounds__(256) void k_piece_sums(const T *__restrict__ gout, G *__restrict__ grad, SumArgs a)
 {
     constexpr int E = Chunk<T>::N, STEP = 4;
-    extern __shared__ uint32_t keys[];                                   // the workgroup's entries, the one before them and the one behind; then their places
+    extern __shared__ uint32_t keys[];                                   // (not WAVE) the workgroup's entries, the one before them and the one behind; then their places
     __shared__ float head[256][E];
     __shared__ uint8_t through[256];
     const int lane = threadIdx.x & ((1 << a.lpr) - 1), group = threadIdx.x >> a.lpr, groups = 256 >> a.lpr, per = groups * SEG;
@@ -404,21 +407,30 @@ __global__ __launch_bounds__(256) void k_piece_sums(const T *__restrict__ gout, 
     const uint32_t none = 0xffffffffu;                                   // a key that no entry has
     for (int64_t b = blockIdx.x; b < a.pieces * a.tiles; b += gridDim.x) {
         const int64_t piece = b / a.tiles, slot = ((b % a.tiles) << a.lpr) + lane, lo = piece * per;
-        for (int i = threadIdx.x; i < per; i += 256) {
-            keys[i + 1] = lo + i < a.n ? a.key[lo + i] : none;
-            places[i] = lo + i < a.n ? a.pos[lo + i] : 0;
+        uint32_t my_key = none, my_place = 0;
+        if constexpr (WAVE) {
+            const int64_t i = lo + group * SEG + lane;                   // lanes 0 .. SEG: this group's and the next entry; lane 63: the one before
+            const int64_t c = lane == 63 ? lo + group * SEG - 1 : i;
+            if ((lane <= SEG || lane == 63) && c >= 0 && c < a.n) my_key = a.key[c];
+            if (lane < SEG && i < a.n) my_place = a.pos[i];
+        } else {
+            for (int i = threadIdx.x; i < per; i += 256) {
+                keys[i + 1] = lo + i < a.n ? a.key[lo + i] : none;
+                places[i] = lo + i < a.n ? a.pos[lo + i] : 0;
+            }
+            if (threadIdx.x == 0) keys[0] = lo > 0 ? a.key[lo - 1] : none;
+            if (threadIdx.x == 64) keys[per + 1] = lo + per < a.n ? a.key[lo + per] : none;
+            __syncthreads();
         }
-        if (threadIdx.x == 0) keys[0] = lo > 0 ? a.key[lo - 1] : none;
-        if (threadIdx.x == 64) keys[per + 1] = lo + per < a.n ? a.key[lo + per] : none;
-        __syncthreads();
-        const uint32_t *k = keys + 1 + group * SEG, *p = places + group * SEG;
+        auto key_of = [&](int i) { return WAVE ? (uint32_t)__builtin_amdgcn_readlane((int)my_key, i < 0 ? 63 : i) : keys[1 + group * SEG + i]; };      // i: -1 .. SEG
+        auto place_of = [&](int i) { return WAVE ? (uint32_t)__builtin_amdgcn_readlane((int)my_place, i) : places[group * SEG + i]; };
         const bool mine = slot < a.slots;
         const Slot<T> at(mine ? slot : 0, a.width);
         u32x4 raw[SEG];
 #pragma unroll
         for (int i = 0; i < SEG; i++) {
             // (absent entries' rows are loaded too where a group has others: one wait for all, and their values are not looked at)
-            const T *row = gout + (int64_t)p[i] * a.ldg + at.j;
+            const T *row = gout + (int64_t)place_of(i) * a.ldg + at.j;
             if constexpr (NARROW) {
                 union { u32x4 v; T e[E]; } u;
                 u.v = u32x4(0);
@@ -431,12 +443,16 @@ __global__ __launch_bounds__(256) void k_piece_sums(const T *__restrict__ gout, 
         float sum[E] = {};                                               // (in the end the tail, where one begins)
         bool first = true, goes_on = false, begins = false, began = false;
         uint32_t last = none;
+        const uint32_t before = key_of(-1);
         // (rolled, the registers moving along: the code that writes a finished sum is there STEP times instead of SEG)
 #pragma unroll 1
         for (int i0 = 0; i0 < SEG; i0 += STEP) {
+            uint32_t k[STEP + 1];
+#pragma unroll
+            for (int i = 0; i <= STEP; i++) k[i] = key_of(i0 + i);
 #pragma unroll
             for (int i = 0; i < STEP; i++) {
-                const uint32_t key = k[i0 + i], next = k[i0 + i + 1];
+                const uint32_t key = k[i], next = k[i + 1];
                 if (key < (uint32_t)a.n_rows) {                          // absent entries are behind all others
                     float f[E];
                     unpack<T>(raw[i], f);
@@ -444,7 +460,7 @@ __global__ __launch_bounds__(256) void k_piece_sums(const T *__restrict__ gout, 
                     for (int e = 0; e < E; e++) sum[e] += f[e];
                     const bool end = i0 + i == SEG - 1;
                     if (end || next != key) {
-                        if (first && k[-1] == key) {
+                        if (first && before == key) {
                             began = true;
                             goes_on = end && next == key;
 #pragma unroll
@@ -556,6 +572,9 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
 }
 
 // ---------------------------------------------------------------------------------------------- log-likelihood of a token
+// The forward pass reads through the caches as usual, so that the backward pass finds in the memory-side cache what that holds of the logits;
+// that pass reads and writes past them (8192 x 32000 bf16, both passes: 174 us so, 212 us with the forward reads non-temporal too, 204 us with
+// the writes alone, 233 us with none).
 // Forward: one read of the row with the running maximum and sum of a softmax. A lane takes BATCH chunks at a time: their maximum first, one
 // rescaling of the sum, then the exponentials. A maximum of -infinity (nothing but excluded classes so far) counts as 0 in the differences,
 // so that they stay -infinity and add 0. LANES lanes take a row; few long rows are cut into parts whose (max, sum) a second launch joins.
@@ -595,7 +614,7 @@ template <class T> __device__ __forceinline__ uint32_t minus_infinities() { retu
 // Chunks c0 .. c1 of a row and its last elements (where `rest`) by LANES lanes. The next BATCH chunks are on their way while these are added:
 // two sets of registers, and loads that are always made (behind the end the last chunk again, its values left out), since a wait behind
 // loads that some lanes may have skipped is a wait for all of them.
-template <class T, bool NT, int LANES> __device__ __forceinline__ MaxSum row_part(const T *x, int64_t c0, int64_t c1, int64_t classes, bool rest, int lane)
+template <class T, int LANES> __device__ __forceinline__ MaxSum row_part(const T *x, int64_t c0, int64_t c1, int64_t classes, bool rest, int lane)
 {
     constexpr int E = Chunk<T>::N, STEP = BATCH * LANES;
     MaxSum a = { -INFINITY, 0.0f };
@@ -604,7 +623,7 @@ template <class T, bool NT, int LANES> __device__ __forceinline__ MaxSum row_par
 #pragma unroll
         for (int i = 0; i < BATCH; i++) {
             const int64_t c = base + i * LANES + lane;
-            v[i] = load_raw<NT>(x + (c < c1 ? c : c1 - 1) * E);
+            v[i] = load_raw<false>(x + (c < c1 ? c : c1 - 1) * E);
         }
     };
     auto add = [&](Set &v, int64_t base) {
@@ -660,7 +679,7 @@ __device__ __forceinline__ void put_loglik(float *logp, float *stats, int64_t t,
     stats[2 * t] = a.m;
     stats[2 * t + 1] = (float)log_sum;
 }
-template <class T, bool NT, int LANES>
+template <class T, int LANES>
 __global__ __launch_bounds__(256) void k_token_loglik(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target,
                                                       float *__restrict__ logp, float *__restrict__ stats)
 {
@@ -674,12 +693,12 @@ __global__ __launch_bounds__(256) void k_token_loglik(const T *__restrict__ logi
             continue;
         }
         const T *x = logits + t * ld;
-        const MaxSum a = join_lanes<LANES>(row_part<T, NT, LANES>(x, 0, classes / Chunk<T>::N, classes, true, lane), ws);
+        const MaxSum a = join_lanes<LANES>(row_part<T, LANES>(x, 0, classes / Chunk<T>::N, classes, true, lane), ws);
         if (lane == 0) put_loglik(logp, stats, t, a, to_float(x[y]));
     }
 }
 // parts of rows, [n][parts] of workspace; parts <= 64
-template <class T, bool NT>
+template <class T>
 __global__ __launch_bounds__(256) void k_token_loglik_parts(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target, int parts,
                                                             MaxSum *__restrict__ out)
 {
@@ -687,7 +706,7 @@ __global__ __launch_bounds__(256) void k_token_loglik_parts(const T *__restrict_
     const int64_t t = blockIdx.x / parts, part = blockIdx.x % parts;
     if (id_at(target, t, classes) < 0) return;
     const int64_t chunks = classes / Chunk<T>::N, step = (chunks + parts - 1) / parts, c0 = part * step < chunks ? part * step : chunks, c1 = c0 + step < chunks ? c0 + step : chunks;
-    const MaxSum a = join_lanes<256>(row_part<T, NT, 256>(logits + t * ld, c0, c1, classes, part == parts - 1, threadIdx.x), ws);
+    const MaxSum a = join_lanes<256>(row_part<T, 256>(logits + t * ld, c0, c1, classes, part == parts - 1, threadIdx.x), ws);
     if (threadIdx.x == 0) out[blockIdx.x] = a;
 }
 template <class T>
@@ -758,7 +777,9 @@ __global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, 
 }
 
 // ---------------------------------------------------------------------------------------------- preference
-// Sums of a sequence in 64 bits: they are differences of log-likelihoods, small next to the terms.
+// A sequence's sum is in 64 bits: it is a small difference of large terms' sums. Three shapes, by the sequences' average length and number:
+// 8 lanes a sequence and 16 pairs a workgroup where they are short, 256 lanes a sequence and a workgroup a pair, and for few long ones parts
+// of sequences, a workgroup each, whose sums the workgroups of the gradient's parts add up again.
 __device__ __forceinline__ double softplus(double h) { return fmax(h, 0.0) + log1p(exp(-fabs(h))); }
 __device__ __forceinline__ double logistic(double h) { return 1.0 / (1.0 + exp(-h)); }
 
@@ -772,76 +793,201 @@ struct PrefArgs {
     const uint8_t *mask;
     const float *weight, *offset;
     float *loss, *pair_loss, *margin, *ratio, *grad;
+    double *losses;                          // workspace: a workgroup's losses
+    double *sums;                            // workspace: [2 pairs][parts][2]
+    int parts;
 };
-__device__ __forceinline__ void seq_range(const PrefArgs &a, int64_t s, int64_t &b, int64_t &e)
+struct Range { int64_t b, e; };
+__device__ __forceinline__ Range sequence(const PrefArgs &a, int64_t s)
 {
-    b = a.seq_ptr[s];
-    e = a.seq_ptr[s + 1];
+    int64_t b = a.seq_ptr[s], e = a.seq_ptr[s + 1];
     b = b < 0 ? 0 : b > a.n ? a.n : b;
     e = e < b ? b : e > a.n ? a.n : e;
+    return { b, e };
 }
-__global__ __launch_bounds__(256) void k_preference_pairs(PrefArgs a)
+__device__ __forceinline__ Range part_of(Range r, int64_t part, int64_t parts)
 {
-    __shared__ double sums[4][2];
-    for (int64_t p = blockIdx.x; p < a.pairs; p += gridDim.x) {
-        double ratio[2], part[2];
-        int64_t from[2], to[2];
-        for (int side = 0; side < 2; side++) {
-            seq_range(a, p + side * a.pairs, from[side], to[side]);
-            double sum = 0, count = 0;
-            for (int64_t t = from[side] + threadIdx.x; t < to[side]; t += 256)
-                if (!a.mask || a.mask[t]) {
-                    sum += (double)a.logp[t] - (a.ref ? (double)a.ref[t] : 0.0);
-                    count += 1;
-                }
-            sum = wave_all(sum, [](double x, double y) { return x + y; });
-            count = wave_all(count, [](double x, double y) { return x + y; });
-            if ((threadIdx.x & 63) == 0) { sums[threadIdx.x >> 6][0] = sum; sums[threadIdx.x >> 6][1] = count; }
-            __syncthreads();
-            sum = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
-            count = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
-            __syncthreads();
-            part[side] = a.mean ? (count > 0 ? 1.0 / count : 0.0) : 1.0;
-            ratio[side] = sum * part[side];
-        }
-        const double h = (double)a.beta * (ratio[0] - ratio[1]) + (a.offset ? (double)a.offset[p] : 0.0), eps = (double)a.smoothing;
-        const double w = (double)a.scale * (a.weight ? (double)a.weight[p] : 1.0);
-        // each term only where its factor is not 0: an infinite margin must not make 0 * infinity of the other one
-        const double loss = (eps < 1 ? (1 - eps) * softplus(-h) : 0.0) + (eps > 0 ? eps * softplus(h) : 0.0);
-        const double slope = w == 0 ? 0.0 : w * (double)a.beta * (eps * logistic(h) - (1 - eps) * logistic(-h));
-        if (threadIdx.x == 0) {
-            a.pair_loss[p] = (float)loss;
-            if (a.margin) a.margin[p] = (float)h;
-            if (a.ratio) { a.ratio[p] = (float)ratio[0]; a.ratio[a.pairs + p] = (float)ratio[1]; }
-        }
-        if (!a.grad) continue;
-        for (int side = 0; side < 2; side++) {
-            const float g = (float)((side ? -slope : slope) * part[side]);
-            for (int64_t t = from[side] + threadIdx.x; t < to[side]; t += 256) a.grad[t] = !a.mask || a.mask[t] ? g : 0.0f;
-        }
-    }
+    const int64_t step = ((r.e - r.b + parts - 1) / parts + 3) / 4 * 4, b = r.b + part * step;
+    return { b < r.e ? b : r.e, b + step < r.e ? b + step : r.e };
 }
-// the sum of the losses, and the gradient of the tokens before the first sequence and behind the last
-__global__ __launch_bounds__(256) void k_preference_total(PrefArgs a)
+struct SeqSum { double sum, count; };
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_at4 __attribute__((aligned(4)));
+typedef uint32_t u32_at1 __attribute__((aligned(1)));
+__device__ __forceinline__ void add_token(SeqSum &s, bool on, float logp, float ref)
 {
-    __shared__ double sums[4];
-    if (blockIdx.x == 0) {
-        double sum = 0;
-        for (int64_t p = threadIdx.x; p < a.pairs; p += 256) {
-            const double w = (double)a.scale * (a.weight ? (double)a.weight[p] : 1.0);
-            if (w != 0) sum += w * (double)a.pair_loss[p];
-        }
-        sum = wave_all(sum, [](double x, double y) { return x + y; });
-        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
-        __syncthreads();
-        if (threadIdx.x == 0) a.loss[0] = (float)((sums[0] + sums[1]) + (sums[2] + sums[3]));
+    if (on) { s.sum += (double)logp - (double)ref; s.count += 1; }
+}
+// lane's share of a range: 4 tokens of every 4 LANES
+template <int LANES> __device__ __forceinline__ SeqSum sum_tokens(const PrefArgs &a, Range r, int lane)
+{
+    SeqSum s = { 0, 0 };
+    int64_t t = r.b + 4 * lane;
+#pragma unroll 2
+    for (; t + 4 <= r.e; t += 4 * LANES) {
+        const f32x4 x = *reinterpret_cast<const f32x4_at4 *>(a.logp + t), y = a.ref ? f32x4(*reinterpret_cast<const f32x4_at4 *>(a.ref + t)) : f32x4(0.0f);
+        const uint32_t m = a.mask ? uint32_t(*reinterpret_cast<const u32_at1 *>(a.mask + t)) : 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < 4; i++) add_token(s, (m >> (8 * i)) & 255, x[i], y[i]);
     }
+    for (; t < r.e; t++) add_token(s, !a.mask || a.mask[t], a.logp[t], a.ref ? a.ref[t] : 0.0f);        // (one lane's, at the end: fewer than 4)
+    return s;
+}
+template <int LANES> __device__ __forceinline__ void put_gradient(const PrefArgs &a, Range r, int lane, float g)
+{
+    int64_t t = r.b + 4 * lane;
+#pragma unroll 2
+    for (; t + 4 <= r.e; t += 4 * LANES) {
+        const uint32_t m = a.mask ? uint32_t(*reinterpret_cast<const u32_at1 *>(a.mask + t)) : 0xffffffffu;
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (m >> (8 * i)) & 255 ? g : 0.0f;
+        *reinterpret_cast<f32x4_at4 *>(a.grad + t) = v;
+    }
+    for (; t < r.e; t++) a.grad[t] = !a.mask || a.mask[t] ? g : 0.0f;
+}
+// over the LANES (a power of 2, 64 at most) lanes of a group
+template <int LANES> __device__ __forceinline__ SeqSum join_sums(SeqSum s)
+{
+#pragma unroll
+    for (int m = LANES / 2; m; m >>= 1) {
+        s.sum += __shfl_xor(s.sum, m);
+        s.count += __shfl_xor(s.count, m);
+    }
+    return s;
+}
+// what one pair comes to; its values are written where `writes`. Returns scale * weight * loss, and the gradients of the two sequences' tokens.
+__device__ __forceinline__ double pair_of(const PrefArgs &a, int64_t p, const SeqSum (&s)[2], float (&g)[2], bool writes)
+{
+    double ratio[2], part[2];
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+        part[side] = a.mean ? (s[side].count > 0 ? 1.0 / s[side].count : 0.0) : 1.0;
+        ratio[side] = s[side].sum * part[side];
+    }
+    const double h = (double)a.beta * (ratio[0] - ratio[1]) + (a.offset ? (double)a.offset[p] : 0.0), eps = (double)a.smoothing;
+    const double w = (double)a.scale * (a.weight ? (double)a.weight[p] : 1.0);
+    // each term only where its factor is not 0: an infinite margin must not make 0 * infinity of the other one
+    const double loss = (eps < 1 ? (1 - eps) * softplus(-h) : 0.0) + (eps > 0 ? eps * softplus(h) : 0.0);
+    const double slope = w == 0 ? 0.0 : w * (double)a.beta * (eps * logistic(h) - (1 - eps) * logistic(-h));
+    g[0] = (float)(slope * part[0]);
+    g[1] = (float)(-slope * part[1]);
+    if (writes) {
+        a.pair_loss[p] = (float)loss;
+        if (a.margin) a.margin[p] = (float)h;
+        if (a.ratio) { a.ratio[p] = (float)ratio[0]; a.ratio[a.pairs + p] = (float)ratio[1]; }
+    }
+    return w == 0 ? 0.0 : w * loss;
+}
+// tokens before the first sequence and behind the last have no gradient
+__device__ __forceinline__ void put_outside(const PrefArgs &a)
+{
     if (!a.grad) return;
-    int64_t first = a.seq_ptr[0], last = a.seq_ptr[2 * a.pairs];
-    first = a.pairs == 0 ? a.n : first < 0 ? 0 : first > a.n ? a.n : first;
+    int64_t first = a.pairs ? a.seq_ptr[0] : a.n, last = a.pairs ? a.seq_ptr[2 * a.pairs] : a.n;
+    first = first < 0 ? 0 : first > a.n ? a.n : first;
     last = last < first ? first : last > a.n ? a.n : last;
-    for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < first; t += gridDim.x * 256ll) a.grad[t] = 0.0f;
-    for (int64_t t = last + blockIdx.x * 256ll + threadIdx.x; t < a.n; t += gridDim.x * 256ll) a.grad[t] = 0.0f;
+    const int64_t step = (int64_t)gridDim.x * blockDim.x, t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    for (int64_t i = t; i < first; i += step) a.grad[i] = 0.0f;
+    for (int64_t i = last + t; i < a.n; i += step) a.grad[i] = 0.0f;
+}
+// 8 lanes a sequence: lanes 0-7 of 16 the preferred one
+constexpr int FEW_PAIRS = 16;                // pairs of a workgroup
+__global__ __launch_bounds__(256) void k_preference_short(PrefArgs a)
+{
+    __shared__ double of_pair[FEW_PAIRS];
+    const int lane = threadIdx.x & 7, side = (threadIdx.x >> 3) & 1, local = threadIdx.x >> 4;
+    double loss = 0;
+    put_outside(a);
+    for (int64_t p0 = (int64_t)blockIdx.x * FEW_PAIRS; p0 < a.pairs; p0 += (int64_t)gridDim.x * FEW_PAIRS) {
+        const int64_t p = p0 + local;
+        const bool here = p < a.pairs;
+        const Range r = here ? sequence(a, p + side * a.pairs) : Range{ 0, 0 };
+        const SeqSum mine = join_sums<8>(sum_tokens<8>(a, r, lane)), other = { __shfl_xor(mine.sum, 8), __shfl_xor(mine.count, 8) };
+        if (!here) continue;
+        const SeqSum both[2] = { side ? other : mine, side ? mine : other };
+        float g[2];
+        loss += pair_of(a, p, both, g, (threadIdx.x & 15) == 0);
+        if (a.grad) put_gradient<8>(a, r, lane, g[side]);
+    }
+    if ((threadIdx.x & 15) == 0) of_pair[local] = loss;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double sum = 0;
+        for (int i = 0; i < FEW_PAIRS; i++) sum += of_pair[i];
+        if (gridDim.x == 1) a.loss[0] = (float)sum;
+        else a.losses[blockIdx.x] = sum;
+    }
+}
+// 256 lanes a sequence
+__global__ __launch_bounds__(512) void k_preference_pairs(PrefArgs a)
+{
+    __shared__ SeqSum waves[8];
+    const int lane = threadIdx.x & 255, side = threadIdx.x >> 8;
+    double loss = 0;
+    put_outside(a);
+    for (int64_t p = blockIdx.x; p < a.pairs; p += gridDim.x) {
+        const Range r = sequence(a, p + side * a.pairs);
+        const SeqSum s = join_sums<64>(sum_tokens<256>(a, r, lane));
+        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = s;
+        __syncthreads();
+        SeqSum both[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            both[i].sum = (waves[4 * i].sum + waves[4 * i + 1].sum) + (waves[4 * i + 2].sum + waves[4 * i + 3].sum);
+            both[i].count = (waves[4 * i].count + waves[4 * i + 1].count) + (waves[4 * i + 2].count + waves[4 * i + 3].count);
+        }
+        float g[2];
+        loss += pair_of(a, p, both, g, threadIdx.x == 0);
+        if (a.grad) put_gradient<256>(a, r, lane, g[side]);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        if (gridDim.x == 1) a.loss[0] = (float)loss;
+        else a.losses[blockIdx.x] = loss;
+    }
+}
+// parts of sequences: their sums, then (64 parts at most) every part's gradient
+__global__ __launch_bounds__(256) void k_preference_part_sums(PrefArgs a)
+{
+    __shared__ SeqSum waves[4];
+    const int64_t s = blockIdx.x / a.parts;
+    const SeqSum x = join_sums<64>(sum_tokens<256>(a, part_of(sequence(a, s), blockIdx.x % a.parts, a.parts), threadIdx.x));
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a.sums[2 * (int64_t)blockIdx.x] = (waves[0].sum + waves[1].sum) + (waves[2].sum + waves[3].sum);
+        a.sums[2 * (int64_t)blockIdx.x + 1] = (waves[0].count + waves[1].count) + (waves[2].count + waves[3].count);
+    }
+}
+__global__ __launch_bounds__(256) void k_preference_part_gradients(PrefArgs a)
+{
+    const int64_t s = blockIdx.x / a.parts, part = blockIdx.x % a.parts, p = s < a.pairs ? s : s - a.pairs;
+    const int lane = threadIdx.x & 63, side = s < a.pairs ? 0 : 1;
+    put_outside(a);
+    SeqSum both[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        both[i] = { 0, 0 };
+        const double *in = a.sums + 2 * ((p + i * a.pairs) * a.parts + lane);
+        if (lane < a.parts) both[i] = { in[0], in[1] };
+        both[i] = join_sums<64>(both[i]);
+    }
+    float g[2];
+    const bool writes = side == 0 && part == 0 && threadIdx.x == 0;
+    const double loss = pair_of(a, p, both, g, writes);
+    if (writes) a.losses[p] = loss;
+    if (a.grad) put_gradient<256>(a, part_of(sequence(a, s), part, a.parts), threadIdx.x, g[side]);
+}
+__global__ __launch_bounds__(256) void k_preference_total(PrefArgs a, int64_t count)
+{
+    __shared__ double waves[4];
+    double sum = 0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < count; i += 256) sum += a.losses[i];
+    sum = wave_all(sum, [](double x, double y) { return x + y; });
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) a.loss[0] = (float)((waves[0] + waves[1]) + (waves[2] + waves[3]));
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -937,6 +1083,22 @@ LoglikPlan loglik_plan(int64_t es, int64_t n, int64_t classes)
 template <class F> int by_lanes(int lanes, F &&f)
 {
     return lanes == 8 ? f(std::integral_constant<int, 8>()) : lanes == 64 ? f(std::integral_constant<int, 64>()) : f(std::integral_constant<int, 256>());
+}
+
+// Short sequences (64 tokens on average) have 8 lanes each, others 256; where that makes fewer than 256 workgroups of sequences of
+// more than 8192 tokens on average, these are cut into parts of 4096 or more, 64 at most and 1024 workgroups in all.
+struct PrefPlan { bool few; int parts; int64_t groups; size_t sums, bytes; };
+PrefPlan preference_plan(int64_t n, int64_t pairs)
+{
+    PrefPlan p = { true, 1, 1, 0, 0 };
+    if (pairs == 0) return p;
+    const int64_t average = n / (2 * pairs);
+    p.few = average <= 64;
+    if (!p.few && pairs < 256 && average > 8192) p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({ 64, average / 4096, 1024 / (2 * pairs) }));
+    p.groups = grid_of(p.few ? ceil_div(pairs, FEW_PAIRS) : pairs);
+    p.sums = p.parts > 1 ? (size_t)(2 * pairs * p.parts) * 16 : 0;
+    p.bytes = p.groups > 1 || p.parts > 1 ? p.sums + (size_t)p.groups * 8 : 0;
+    return p;
 }
 
 }  // namespace
@@ -1052,8 +1214,12 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
                 });
         if (n_ids == 0) return 0;
         const SumArgs a = { key[cur], pos[cur], n_ids, n_rows, width, ld_grad_out, ld_grad, plan.slots, plan.tiles, plan.pieces, scale, accumulate != 0, plan.lpr, part };
-        hipLaunchKernelGGL((k_piece_sums<T, G, NT, NARROW>), dim3(grid_of(plan.pieces * plan.tiles)), dim3(256), (2 * (256 >> plan.lpr) * SEG + 2) * sizeof(uint32_t),
-                           st, (const T *)grad_out, out, a);
+        by_flag(plan.lpr == 6, [&](auto wave) {
+            constexpr bool WAVE = decltype(wave)::value && !NARROW;
+            hipLaunchKernelGGL((k_piece_sums<T, G, NT, NARROW, WAVE>), dim3(grid_of(plan.pieces * plan.tiles)), dim3(256),
+                               WAVE ? 0 : (2 * (256 >> plan.lpr) * SEG + 2) * sizeof(uint32_t), st, (const T *)grad_out, out, a);
+            return 0;
+        });
         if (plan.pieces > 1) hipLaunchKernelGGL((k_piece_join<T, G, NT, NARROW>), dim3(grid_of((plan.pieces - 1) * plan.tiles)), dim3(256), 0, st, out, a);
         return 0;
     };
@@ -1096,23 +1262,19 @@ int mlx_token_loglik(int32_t device, void *stream, int32_t type, const void *log
     if (on.rc) return on.rc;
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
-        return by_flag(streams(n_tokens, n_classes, es), [&](auto nt) {
-            constexpr bool NT = decltype(nt)::value;
-            hipStream_t st = (hipStream_t)stream;
-            const T *x = (const T *)logits;
-            const Ids y = { target, id_type == MLX_I64 };
-            if (plan.parts > 1) {
-                hipLaunchKernelGGL((k_token_loglik_parts<T, NT>), dim3((unsigned)(n_tokens * plan.parts)), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
-                                   (MaxSum *)workspace);
-                hipLaunchKernelGGL((k_token_loglik_join<T>), dim3((unsigned)n_tokens), dim3(64), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
-                                   (const MaxSum *)workspace, logp, stats);
-            } else
-                by_lanes(plan.lanes, [&](auto l) {
-                    constexpr int LANES = decltype(l)::value;
-                    hipLaunchKernelGGL((k_token_loglik<T, NT, LANES>), dim3(grid_of(ceil_div(n_tokens, 256 / LANES))), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, logp,
-                                       stats);
-                    return 0;
-                });
+        hipStream_t st = (hipStream_t)stream;
+        const T *x = (const T *)logits;
+        const Ids y = { target, id_type == MLX_I64 };
+        if (plan.parts > 1) {
+            hipLaunchKernelGGL((k_token_loglik_parts<T>), dim3((unsigned)(n_tokens * plan.parts)), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
+                               (MaxSum *)workspace);
+            hipLaunchKernelGGL((k_token_loglik_join<T>), dim3((unsigned)n_tokens), dim3(64), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
+                               (const MaxSum *)workspace, logp, stats);
+            return 0;
+        }
+        return by_lanes(plan.lanes, [&](auto l) {
+            constexpr int LANES = decltype(l)::value;
+            hipLaunchKernelGGL((k_token_loglik<T, LANES>), dim3(grid_of(ceil_div(n_tokens, 256 / LANES))), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, logp, stats);
             return 0;
         });
     });
@@ -1160,7 +1322,7 @@ int mlx_preference_loss_workspace(int64_t n_tokens, int64_t n_pairs, size_t *byt
     const char *who = "mlx_preference_loss_workspace";
     MLX_REFUSE(!bytes, "%s: bytes is NULL", who);
     MLX_REFUSE(n_tokens < 0 || n_tokens > MOST || n_pairs < 0 || n_pairs > MOST / 2, "%s: bad sizes", who);
-    *bytes = 0;
+    *bytes = preference_plan(n_tokens, n_pairs).bytes;
     return MLX_OK;
 }
 
@@ -1176,8 +1338,8 @@ int mlx_preference_loss(int32_t device, void *stream, const float *logp, const f
     MLX_REFUSE((n_tokens > 0 && !logp) || !seq_ptr || !loss || (n_pairs > 0 && !pair_loss), "%s: logp, seq_ptr, loss or pair_loss is NULL", who);
     MLX_REFUSE(((uintptr_t)logp | (uintptr_t)ref_logp | (uintptr_t)weight | (uintptr_t)offset | (uintptr_t)loss | (uintptr_t)pair_loss | (uintptr_t)margin |
                 (uintptr_t)ratio | (uintptr_t)grad) % 4 || (uintptr_t)seq_ptr % 8, "%s: a pointer is not aligned to its elements", who);
-    size_t need;
-    if (int rc = mlx_preference_loss_workspace(n_tokens, n_pairs, &need)) return rc;
+    const PrefPlan plan = preference_plan(n_tokens, n_pairs);
+    const size_t need = plan.bytes;
     MLX_REFUSE(workspace_bytes < need, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, need);
     MLX_REFUSE(need && (!workspace || (uintptr_t)workspace % 256), "%s: workspace is NULL or not aligned to 256 bytes", who);
     const struct { const void *p; int64_t n; } in[] = { { logp, 4 * n_tokens }, { ref_logp, 4 * n_tokens }, { seq_ptr, 8 * (2 * n_pairs + 1) }, { mask, n_tokens },
@@ -1191,9 +1353,15 @@ int mlx_preference_loss(int32_t device, void *stream, const float *logp, const f
     }
     OnDevice on(device);
     if (on.rc) return on.rc;
-    const PrefArgs a = { logp, ref_logp, n_tokens, seq_ptr, n_pairs, beta, smoothing, scale, mean != 0, mask, weight, offset, loss, pair_loss, margin, ratio, grad };
-    if (n_pairs > 0) hipLaunchKernelGGL(k_preference_pairs, dim3(grid_of(n_pairs)), dim3(256), 0, (hipStream_t)stream, a);
-    hipLaunchKernelGGL(k_preference_total, dim3(64), dim3(256), 0, (hipStream_t)stream, a);
+    const PrefArgs a = { logp, ref_logp, n_tokens, seq_ptr, n_pairs, beta, smoothing, scale, mean != 0, mask, weight, offset, loss, pair_loss, margin, ratio, grad,
+                         (double *)((char *)workspace + plan.sums), (double *)workspace, plan.parts };
+    hipStream_t st = (hipStream_t)stream;
+    if (plan.parts > 1) {
+        hipLaunchKernelGGL(k_preference_part_sums, dim3((unsigned)(2 * n_pairs * plan.parts)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(k_preference_part_gradients, dim3((unsigned)(2 * n_pairs * plan.parts)), dim3(256), 0, st, a);
+    } else if (plan.few) hipLaunchKernelGGL(k_preference_short, dim3((unsigned)plan.groups), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_preference_pairs, dim3((unsigned)plan.groups), dim3(512), 0, st, a);
+    if (plan.groups > 1 || plan.parts > 1) hipLaunchKernelGGL(k_preference_total, dim3(1), dim3(256), 0, st, a, plan.groups);
     return launched(who);
 }
 
