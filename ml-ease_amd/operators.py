@@ -71,6 +71,10 @@ class HipOperators:
         self._at = torch.device("cuda", self.device)
         self._types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
         self._id_types = {torch.int32: 0, torch.int64: 1}
+        self._f32 = torch.float32
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # the stream's handle without the object around it: 2 us of a call
+        at, device = self._at, self.device
+        self._stream = (lambda: raw(device)) if raw else (lambda: torch.cuda.current_stream(at).cuda_stream)
 
     # -- checks -----------------------------------------------------------------------------------
     def _matrix(self, t, what):
@@ -97,12 +101,15 @@ class HipOperators:
             raise ValueError("%s must be a vector of %sint32 or int64, not %s %s" % (what, "" if n is None else "%d " % n, tuple(t.shape), t.dtype))
         return self._vector(t, what, t.shape[0], t.dtype), self._id_types[t.dtype]
 
-    def _output(self, out, what, shape, dtype):
+    def _output(self, out, shape, dtype):
+        """(tensor, pointer, ld) of a new matrix, or of the caller's."""
         if out is None:
-            return self._torch.empty(shape, dtype=dtype, device=self._at)
+            out = self._torch.empty(shape, dtype=dtype, device=self._at)
+            return out, out.data_ptr(), shape[1]
         if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
-            raise ValueError("%s must be %s %s, not %s %s" % (what, tuple(shape), dtype, tuple(out.shape), out.dtype))
-        return out
+            raise ValueError("out must be %s %s, not %s %s" % (tuple(shape), dtype, tuple(out.shape), out.dtype))
+        p, ld = self._matrix(out, "out")
+        return out, p, ld
 
     def _workspace(self, query, *sizes):
         need = C.c_size_t()
@@ -111,9 +118,6 @@ class HipOperators:
             return None, None, 0
         w = self._torch.empty(need.value, dtype=self._torch.uint8, device=self._at)      # torch's blocks are aligned to 512 bytes
         return w, w.data_ptr(), need.value
-
-    def _stream(self):
-        return self._torch.cuda.current_stream(self._at).cuda_stream
 
     def _ck(self, rc):
         if rc != 0:
@@ -125,9 +129,9 @@ class HipOperators:
         tp, ld = self._matrix(table, "table")
         ip, it = self._ids(ids, "ids")
         rows, width = table.shape
-        out = self._output(out, "out", (ids.shape[0], width), table.dtype)
-        op, ldo = self._matrix(out, "out")
-        self._ck(self.L.mlx_embedding_lookup(self.device, self._stream(), self._types[table.dtype], tp, rows, width, ld, it, ip, ids.shape[0], scale, op, ldo))
+        n = ids.shape[0]
+        out, op, ldo = self._output(out, (n, width), table.dtype)
+        self._ck(self.L.mlx_embedding_lookup(self.device, self._stream(), self._types[table.dtype], tp, rows, width, ld, it, ip, n, scale, op, ldo))
         return out
 
     def embedding_gradient(self, grad_out, ids, n_rows: int, scale: float = 1.0, out=None, accumulate: bool = False, dtype=None):
@@ -141,8 +145,7 @@ class HipOperators:
         dtype = dtype or (grad_out.dtype if out is None else out.dtype)
         if dtype not in self._types:
             raise ValueError("grad must be of grad_out's type or float32, not %s" % dtype)
-        out = self._output(out, "out", (n_rows, width), dtype)
-        op, ldo = self._matrix(out, "out")
+        out, op, ldo = self._output(out, (n_rows, width), dtype)
         keep, wp, wb = self._workspace(self.L.mlx_embedding_gradient_workspace, n_rows, width, n)
         self._ck(self.L.mlx_embedding_gradient(self.device, self._stream(), self._types[grad_out.dtype], gp, ldg, it, ip, n, scale, bool(accumulate),
                                                self._types[dtype], op, n_rows, width, ldo, wp, wb))
@@ -155,8 +158,7 @@ class HipOperators:
         lp, ld = self._matrix(logits, "logits")
         n, classes = logits.shape
         ip, it = self._ids(target, "target", n)
-        f32 = self._torch.float32
-        logp, stats = self._output(None, "logp", (n,), f32), self._output(None, "stats", (n, 2), f32)
+        logp, stats = self._torch.empty(n, dtype=self._f32, device=self._at), self._torch.empty((n, 2), dtype=self._f32, device=self._at)
         keep, wp, wb = self._workspace(self.L.mlx_token_loglik_workspace, n, classes)
         self._ck(self.L.mlx_token_loglik(self.device, self._stream(), self._types[logits.dtype], lp, n, classes, ld, it, ip, logp.data_ptr(), stats.data_ptr(), wp, wb))
         return logp, stats
@@ -166,13 +168,11 @@ class HipOperators:
         lp, ld = self._matrix(logits, "logits")
         n, classes = logits.shape
         ip, it = self._ids(target, "target", n)
-        f32 = self._torch.float32
-        gp = self._vector(grad_logp, "grad_logp", n, f32)
+        gp = self._vector(grad_logp, "grad_logp", n, self._f32)
         if tuple(stats.shape) != (n, 2) or not stats.is_contiguous():
             raise ValueError("stats must be what token_loglik gave for these logits, [%d, 2]" % n)
-        sp = self._vector(stats.view(-1), "stats", 2 * n, f32)
-        out = self._output(out, "out", (n, classes), logits.dtype)
-        op, ldo = self._matrix(out, "out")
+        sp = self._vector(stats.view(-1), "stats", 2 * n, self._f32)
+        out, op, ldo = self._output(out, (n, classes), logits.dtype)
         self._ck(self.L.mlx_token_loglik_gradient(self.device, self._stream(), self._types[logits.dtype], lp, n, classes, ld, it, ip, sp, gp, op, ldo))
         return out
 
@@ -183,7 +183,7 @@ class HipOperators:
         are the preferred ones. logp, ref_logp (or None) [n] float32, seq_ptr [2 pairs + 1] int64, mask (or None) [n] bool / uint8, weight, offset
         (or None) [pairs] float32. Returns loss = sum of scale * weight * pair_loss, pair_loss, margin [pairs], ratio [2 pairs] and grad [n]
         (None where grad=False)."""
-        torch, f32 = self._torch, self._torch.float32
+        torch, f32 = self._torch, self._f32
         if seq_ptr.dim() != 1 or seq_ptr.shape[0] % 2 != 1:
             raise ValueError("seq_ptr must be a vector of 2 * pairs + 1 int64, not %s" % (tuple(seq_ptr.shape),))
         n, pairs = logp.numel(), (seq_ptr.shape[0] - 1) // 2
@@ -192,9 +192,12 @@ class HipOperators:
         mp = None if mask is None else self._vector(mask, "mask", n, torch.uint8 if mask.dtype == torch.uint8 else torch.bool)
         wp = None if weight is None else self._vector(weight, "weight", pairs, f32)
         fp = None if offset is None else self._vector(offset, "offset", pairs, f32)
-        loss, pair_loss, margin = self._output(None, "loss", (), f32), self._output(None, "pair_loss", (pairs,), f32), self._output(None, "margin", (pairs,), f32)
-        ratio, g = self._output(None, "ratio", (2 * pairs,), f32), self._output(None, "grad", (n,), f32) if grad else None
+        # the few values of every pair in one block, the gradient in one of its own
+        few = torch.empty(4 * pairs + 1, dtype=f32, device=self._at)
+        ratio, pair_loss, margin, loss = few.split((2 * pairs, pairs, pairs, 1))
+        at = few.data_ptr()
+        g = torch.empty(n, dtype=f32, device=self._at) if grad else None
         keep, kp, kb = self._workspace(self.L.mlx_preference_loss_workspace, n, pairs)
-        self._ck(self.L.mlx_preference_loss(self.device, self._stream(), lp, rp, n, qp, pairs, beta, smoothing, scale, bool(mean), mp, wp, fp, loss.data_ptr(),
-                                            pair_loss.data_ptr(), margin.data_ptr(), ratio.data_ptr(), None if g is None else g.data_ptr(), kp, kb))
-        return PreferenceResult(loss, pair_loss, margin, ratio, g)
+        self._ck(self.L.mlx_preference_loss(self.device, self._stream(), lp, rp, n, qp, pairs, beta, smoothing, scale, bool(mean), mp, wp, fp, at + 16 * pairs,
+                                            at + 8 * pairs, at + 12 * pairs, at, None if g is None else g.data_ptr(), kp, kb))
+        return PreferenceResult(loss.view(()), pair_loss, margin, ratio, g)

@@ -549,7 +549,8 @@ def pair_data(g, lengths, masked, behind=0, before=0):
     return logp, ref, seq, mask
 
 
-LENGTHS = [[1, 1], [0, 0], [0, 5], [7, 0], [3, 4, 5, 6], [1000, 3, 0, 64, 65, 257], [5000, 70000], [40] * 200, [1] * 2002]
+LENGTHS = [[1, 1], [0, 0], [0, 5], [7, 0], [3, 4, 5, 6], [1000, 3, 0, 64, 65, 257], [5000, 70000], [40] * 200, [1] * 2002, [20000, 0, 7, 90001], [65] * 60, [600001, 300002],
+           [9000, 8500, 8000, 10001, 1, 33000]]
 
 
 @gpu
