@@ -616,12 +616,12 @@ template <class T> __device__ __forceinline__ uint32_t minus_infinities() { retu
 // loads that some lanes may have skipped is a wait for all of them.
 template <class T, int LANES> __device__ __forceinline__ MaxSum row_part(const T *x, int64_t c0, int64_t c1, int64_t classes, bool rest, int lane)
 {
-    constexpr int E = Chunk<T>::N, STEP = BATCH * LANES;
+    constexpr int E = Chunk<T>::N, B = LANES == 1024 ? BATCH / 2 : BATCH, STEP = B * LANES;       // (1024 lanes have 128 registers each)
     MaxSum a = { -INFINITY, 0.0f };
-    typedef u32x4 Set[BATCH];
+    typedef u32x4 Set[B];
     auto fetch = [&](Set &v, int64_t base) {
 #pragma unroll
-        for (int i = 0; i < BATCH; i++) {
+        for (int i = 0; i < B; i++) {
             const int64_t c = base + i * LANES + lane;
             v[i] = load_raw<false>(x + (c < c1 ? c : c1 - 1) * E);
         }
@@ -629,11 +629,11 @@ template <class T, int LANES> __device__ __forceinline__ MaxSum row_part(const T
     auto add = [&](Set &v, int64_t base) {
         if (base + STEP > c1)
 #pragma unroll
-            for (int i = 0; i < BATCH; i++)
+            for (int i = 0; i < B; i++)
                 if (base + i * LANES + lane >= c1) v[i] = u32x4(minus_infinities<T>());
-        float f[BATCH * E];
+        float f[B * E];
 #pragma unroll
-        for (int i = 0; i < BATCH; i++) unpack<T>(v[i], f + i * E);
+        for (int i = 0; i < B; i++) unpack<T>(v[i], f + i * E);
         add_values(a, f);
     };
     if (c0 < c1) {
@@ -680,11 +680,11 @@ __device__ __forceinline__ void put_loglik(float *logp, float *stats, int64_t t,
     stats[2 * t + 1] = (float)log_sum;
 }
 template <class T, int LANES>
-__global__ __launch_bounds__(256) void k_token_loglik(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target,
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_token_loglik(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target,
                                                       float *__restrict__ logp, float *__restrict__ stats)
 {
-    constexpr int ROWS = 256 / LANES;
-    __shared__ MaxSum ws[4];
+    constexpr int ROWS = LANES < 256 ? 256 / LANES : 1;
+    __shared__ MaxSum ws[LANES < 64 ? 1 : LANES / 64];
     const int lane = threadIdx.x & (LANES - 1);
     for (int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; t < n; t += (int64_t)gridDim.x * ROWS) {
         const int64_t y = id_at(target, t, classes);
@@ -1068,15 +1068,20 @@ GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
     return g;
 }
 
-// Lanes of a row: enough that a lane has a few chunks, 8 at least. Rows are cut into parts where they are too few to fill the chip:
-// parts of 4 chunks a lane or more, 64 at most (the lanes of the wave that joins them), 512 workgroups in all.
-struct LoglikPlan { int lanes, parts; size_t bytes; };
+// Lanes of a row: enough that a lane has a few chunks, 8 at least; 1024 where the rows are too few to fill the chip with 256 each. The backward
+// pass cuts its rows into parts then (of BATCH chunks a lane or more, 512 workgroups in all); the forward pass does so only where a row has more
+// than LONG_ROW classes, since it needs a second launch to join the parts (64 at most: a wave's lanes): 32 rows of 128000 bf16 take 11 us of one
+// compute unit each, bound by the exponentials, and 5.8 + 3.3 us and a launch more in 16 parts.
+constexpr int64_t LONG_ROW = 160000;
+struct LoglikPlan { int lanes, parts, grad_lanes, grad_parts; size_t bytes; };
 LoglikPlan loglik_plan(int64_t es, int64_t n, int64_t classes)
 {
     LoglikPlan p;
     const int64_t chunks = classes * es / 16;
-    p.lanes = chunks <= 8 * BATCH ? 8 : chunks <= 64 * BATCH ? 64 : 256;
-    p.parts = n >= 512 || n == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({ 64, ceil_div(512, n), chunks / (256 * BATCH) }));
+    p.grad_lanes = p.lanes = chunks <= 8 * BATCH ? 8 : chunks <= 64 * BATCH ? 64 : 256;
+    p.grad_parts = n >= 512 || n == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({ 64, ceil_div(512, n), chunks / (256 * BATCH) }));
+    p.parts = classes > LONG_ROW ? p.grad_parts : 1;
+    if (n <= 512 && p.grad_parts > 1) p.lanes = 1024;
     p.bytes = p.parts > 1 ? (size_t)(n * p.parts) * sizeof(MaxSum) : 0;
     return p;
 }
@@ -1272,6 +1277,10 @@ int mlx_token_loglik(int32_t device, void *stream, int32_t type, const void *log
                                (const MaxSum *)workspace, logp, stats);
             return 0;
         }
+        if (plan.lanes == 1024) {
+            hipLaunchKernelGGL((k_token_loglik<T, 1024>), dim3((unsigned)n_tokens), dim3(1024), 0, st, x, n_tokens, n_classes, ld_logits, y, logp, stats);
+            return 0;
+        }
         return by_lanes(plan.lanes, [&](auto l) {
             constexpr int LANES = decltype(l)::value;
             hipLaunchKernelGGL((k_token_loglik<T, LANES>), dim3(grid_of(ceil_div(n_tokens, 256 / LANES))), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, logp, stats);
@@ -1305,11 +1314,11 @@ int mlx_token_loglik_gradient(int32_t device, void *stream, int32_t type, const 
         typedef decltype(t) T;
         return by_flag(streams(n_tokens, n_classes, es), [&](auto nt) {
             const LoglikPlan plan = loglik_plan(es, n_tokens, n_classes);
-            return by_lanes(plan.lanes, [&](auto l) {
+            return by_lanes(plan.grad_lanes, [&](auto l) {
                 constexpr int LANES = decltype(l)::value;
-                hipLaunchKernelGGL((k_token_loglik_gradient<T, nt.value, LANES>), dim3(grid_of(ceil_div(n_tokens * plan.parts, 256 / LANES))), dim3(256), 0, (hipStream_t)stream,
+                hipLaunchKernelGGL((k_token_loglik_gradient<T, nt.value, LANES>), dim3(grid_of(ceil_div(n_tokens * plan.grad_parts, 256 / LANES))), dim3(256), 0, (hipStream_t)stream,
                                    (const T *)logits, n_tokens, n_classes, ld_logits, Ids{ target, id_type == MLX_I64 }, stats, grad_logp, (T *)dlogits, ld_dlogits,
-                                   (int64_t)plan.parts);
+                                   (int64_t)plan.grad_parts);
                 return 0;
             });
         });
