@@ -521,7 +521,8 @@ __global__ __launch_bounds__(256) void k_piece_sums(const T *__restrict__ gout, 
 }
 
 // Ids that cross the border of two pieces: the workgroup of the piece in which one begins adds the sums of its pieces, every group of lanes
-// each groups-th of them, then the groups' sums by halves.
+// each groups-th of them, then the groups' sums by halves. (512 lanes a workgroup: an id of 100000 rows of 256 90 us instead of 120, and everything
+// else 5 to 10 % slower, the workgroups that find nothing to join being most of them.)
 template <class T, class G, bool NT, bool NARROW>
 __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArgs a)
 {
@@ -546,7 +547,7 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
         float sum[E] = {};
         if (mine) {
             // pieces piece + 1 .. piece + count, and as number 0 the tail of `piece`
-#pragma unroll 4
+#pragma unroll 8
             for (int64_t q = group; q <= count; q += groups) {
                 const float *in = a.part + (((piece + q) * 2 + (q == 0)) * a.slots + slot) * E;
 #pragma unroll
@@ -610,10 +611,9 @@ template <int N> __device__ __forceinline__ void add_values(MaxSum &a, const flo
     for (int i = 0; i < N; i++) more[i & 3] += exp_of(f[i] - r);
     a = { m, s + ((more[0] + more[1]) + (more[2] + more[3])) };
 }
-template <class T> __device__ __forceinline__ uint32_t minus_infinities() { return sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, __bf16> ? 0xFF80FF80u : 0xFC00FC00u; }
 // Chunks c0 .. c1 of a row and its last elements (where `rest`) by LANES lanes. The next BATCH chunks are on their way while these are added:
-// two sets of registers, and loads that are always made (behind the end the last chunk again, its values left out), since a wait behind
-// loads that some lanes may have skipped is a wait for all of them.
+// two sets of registers, and loads that are always made (behind the end the last chunk again, not looked at), since a wait behind loads that
+// some lanes may have skipped is a wait for all of them.
 template <class T, int LANES> __device__ __forceinline__ MaxSum row_part(const T *x, int64_t c0, int64_t c1, int64_t classes, bool rest, int lane)
 {
     constexpr int E = Chunk<T>::N, B = LANES == 1024 ? BATCH / 2 : BATCH, STEP = B * LANES;       // (1024 lanes have 128 registers each)
@@ -627,10 +627,16 @@ template <class T, int LANES> __device__ __forceinline__ MaxSum row_part(const T
         }
     };
     auto add = [&](Set &v, int64_t base) {
-        if (base + STEP > c1)
+        if (base + STEP > c1) {                                          // the row's last chunks: one at a time, none for lanes behind the end
 #pragma unroll
             for (int i = 0; i < B; i++)
-                if (base + i * LANES + lane >= c1) v[i] = u32x4(minus_infinities<T>());
+                if (base + i * LANES + lane < c1) {
+                    float f[E];
+                    unpack<T>(v[i], f);
+                    add_values(a, f);
+                }
+            return;
+        }
         float f[B * E];
 #pragma unroll
         for (int i = 0; i < B; i++) unpack<T>(v[i], f + i * E);
@@ -778,7 +784,7 @@ __global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, 
 
 // ---------------------------------------------------------------------------------------------- preference
 // A sequence's sum is in 64 bits: it is a small difference of large terms' sums. Three shapes, by the sequences' average length and number:
-// 8 lanes a sequence and 16 pairs a workgroup where they are short, 256 lanes a sequence and a workgroup a pair, and for few long ones parts
+// 1 or 8 lanes a sequence where they are short, 256 lanes a sequence and a workgroup a pair, and for few long ones parts
 // of sequences, a workgroup each, whose sums the workgroups of the gradient's parts add up again.
 __device__ __forceinline__ double softplus(double h) { return fmax(h, 0.0) + log1p(exp(-fabs(h))); }
 __device__ __forceinline__ double logistic(double h) { return 1.0 / (1.0 + exp(-h)); }
@@ -890,30 +896,33 @@ __device__ __forceinline__ void put_outside(const PrefArgs &a)
     for (int64_t i = t; i < first; i += step) a.grad[i] = 0.0f;
     for (int64_t i = last + t; i < a.n; i += step) a.grad[i] = 0.0f;
 }
-// 8 lanes a sequence: lanes 0-7 of 16 the preferred one
-constexpr int FEW_PAIRS = 16;                // pairs of a workgroup
+// LANES lanes a sequence, the preferred one's first; 128 / LANES pairs a workgroup
+template <int LANES>
 __global__ __launch_bounds__(256) void k_preference_short(PrefArgs a)
 {
-    __shared__ double of_pair[FEW_PAIRS];
-    const int lane = threadIdx.x & 7, side = (threadIdx.x >> 3) & 1, local = threadIdx.x >> 4;
+    constexpr int PAIRS = 128 / LANES;
+    __shared__ double waves[4];
+    const int lane = threadIdx.x % LANES, side = threadIdx.x / LANES % 2, local = threadIdx.x / (2 * LANES);
+    const bool one = threadIdx.x % (2 * LANES) == 0;                     // the lane that counts for the pair
     double loss = 0;
     put_outside(a);
-    for (int64_t p0 = (int64_t)blockIdx.x * FEW_PAIRS; p0 < a.pairs; p0 += (int64_t)gridDim.x * FEW_PAIRS) {
+    for (int64_t p0 = (int64_t)blockIdx.x * PAIRS; p0 < a.pairs; p0 += (int64_t)gridDim.x * PAIRS) {
         const int64_t p = p0 + local;
         const bool here = p < a.pairs;
         const Range r = here ? sequence(a, p + side * a.pairs) : Range{ 0, 0 };
-        const SeqSum mine = join_sums<8>(sum_tokens<8>(a, r, lane)), other = { __shfl_xor(mine.sum, 8), __shfl_xor(mine.count, 8) };
+        const SeqSum mine = join_sums<LANES>(sum_tokens<LANES>(a, r, lane)), other = { __shfl_xor(mine.sum, LANES), __shfl_xor(mine.count, LANES) };
         if (!here) continue;
         const SeqSum both[2] = { side ? other : mine, side ? mine : other };
         float g[2];
-        loss += pair_of(a, p, both, g, (threadIdx.x & 15) == 0);
-        if (a.grad) put_gradient<8>(a, r, lane, g[side]);
+        const double x = pair_of(a, p, both, g, one);
+        if (one) loss += x;
+        if (a.grad) put_gradient<LANES>(a, r, lane, g[side]);
     }
-    if ((threadIdx.x & 15) == 0) of_pair[local] = loss;
+    loss = wave_all(loss, [](double x, double y) { return x + y; });
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = loss;
     __syncthreads();
     if (threadIdx.x == 0) {
-        double sum = 0;
-        for (int i = 0; i < FEW_PAIRS; i++) sum += of_pair[i];
+        const double sum = (waves[0] + waves[1]) + (waves[2] + waves[3]);
         if (gridDim.x == 1) a.loss[0] = (float)sum;
         else a.losses[blockIdx.x] = sum;
     }
@@ -1078,7 +1087,10 @@ LoglikPlan loglik_plan(int64_t es, int64_t n, int64_t classes)
 {
     LoglikPlan p;
     const int64_t chunks = classes * es / 16;
-    p.grad_lanes = p.lanes = chunks <= 8 * BATCH ? 8 : chunks <= 64 * BATCH ? 64 : 256;
+    p.lanes = 8;
+    while (p.lanes < 64 && chunks > p.lanes * BATCH) p.lanes *= 2;
+    if (chunks > p.lanes * BATCH) p.lanes = 256;
+    p.grad_lanes = p.lanes;
     p.grad_parts = n >= 512 || n == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({ 64, ceil_div(512, n), chunks / (256 * BATCH) }));
     p.parts = classes > LONG_ROW ? p.grad_parts : 1;
     if (n <= 512 && p.grad_parts > 1) p.lanes = 1024;
@@ -1087,20 +1099,22 @@ LoglikPlan loglik_plan(int64_t es, int64_t n, int64_t classes)
 }
 template <class F> int by_lanes(int lanes, F &&f)
 {
-    return lanes == 8 ? f(std::integral_constant<int, 8>()) : lanes == 64 ? f(std::integral_constant<int, 64>()) : f(std::integral_constant<int, 256>());
+    return lanes == 8 ? f(std::integral_constant<int, 8>()) : lanes == 16 ? f(std::integral_constant<int, 16>()) : lanes == 32 ? f(std::integral_constant<int, 32>()) :
+           lanes == 64 ? f(std::integral_constant<int, 64>()) : f(std::integral_constant<int, 256>());
 }
 
-// Short sequences (64 tokens on average) have 8 lanes each, others 256; where that makes fewer than 256 workgroups of sequences of
+// Short sequences (4, 64 tokens on average) have 1, 8 lanes each, others 256 (of one million pairs of one token 8 lanes each take 249 us: the pair's
+// logarithm and exponentials in 64 bits are every lane's work); where that makes fewer than 256 workgroups of sequences of
 // more than 8192 tokens on average, these are cut into parts of 4096 or more, 64 at most and 1024 workgroups in all.
-struct PrefPlan { bool few; int parts; int64_t groups; size_t sums, bytes; };
+struct PrefPlan { int lanes, parts; int64_t groups; size_t sums, bytes; };
 PrefPlan preference_plan(int64_t n, int64_t pairs)
 {
-    PrefPlan p = { true, 1, 1, 0, 0 };
+    PrefPlan p = { 8, 1, 1, 0, 0 };
     if (pairs == 0) return p;
     const int64_t average = n / (2 * pairs);
-    p.few = average <= 64;
-    if (!p.few && pairs < 256 && average > 8192) p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({ 64, average / 4096, 1024 / (2 * pairs) }));
-    p.groups = grid_of(p.few ? ceil_div(pairs, FEW_PAIRS) : pairs);
+    p.lanes = average <= 4 ? 1 : average <= 64 ? 8 : 256;
+    if (p.lanes == 256 && pairs < 256 && average > 8192) p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({ 64, average / 4096, 1024 / (2 * pairs) }));
+    p.groups = grid_of(p.lanes < 256 ? ceil_div(pairs, 128 / p.lanes) : pairs);
     p.sums = p.parts > 1 ? (size_t)(2 * pairs * p.parts) * 16 : 0;
     p.bytes = p.groups > 1 || p.parts > 1 ? p.sums + (size_t)p.groups * 8 : 0;
     return p;
@@ -1312,8 +1326,8 @@ int mlx_token_loglik_gradient(int32_t device, void *stream, int32_t type, const 
     if (on.rc) return on.rc;
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
-        return by_flag(streams(n_tokens, n_classes, es), [&](auto nt) {
-            const LoglikPlan plan = loglik_plan(es, n_tokens, n_classes);
+        const LoglikPlan plan = loglik_plan(es, n_tokens, n_classes);
+        return by_flag(plan.grad_lanes == 256 && streams(n_tokens, n_classes, es), [&](auto nt) {
             return by_lanes(plan.grad_lanes, [&](auto l) {
                 constexpr int LANES = decltype(l)::value;
                 hipLaunchKernelGGL((k_token_loglik_gradient<T, nt.value, LANES>), dim3(grid_of(ceil_div(n_tokens * plan.grad_parts, 256 / LANES))), dim3(256), 0, (hipStream_t)stream,
@@ -1368,7 +1382,8 @@ int mlx_preference_loss(int32_t device, void *stream, const float *logp, const f
     if (plan.parts > 1) {
         hipLaunchKernelGGL(k_preference_part_sums, dim3((unsigned)(2 * n_pairs * plan.parts)), dim3(256), 0, st, a);
         hipLaunchKernelGGL(k_preference_part_gradients, dim3((unsigned)(2 * n_pairs * plan.parts)), dim3(256), 0, st, a);
-    } else if (plan.few) hipLaunchKernelGGL(k_preference_short, dim3((unsigned)plan.groups), dim3(256), 0, st, a);
+    } else if (plan.lanes == 1) hipLaunchKernelGGL(k_preference_short<1>, dim3((unsigned)plan.groups), dim3(256), 0, st, a);
+    else if (plan.lanes == 8) hipLaunchKernelGGL(k_preference_short<8>, dim3((unsigned)plan.groups), dim3(256), 0, st, a);
     else hipLaunchKernelGGL(k_preference_pairs, dim3((unsigned)plan.groups), dim3(512), 0, st, a);
     if (plan.groups > 1 || plan.parts > 1) hipLaunchKernelGGL(k_preference_total, dim3(1), dim3(256), 0, st, a, plan.groups);
     return launched(who);
