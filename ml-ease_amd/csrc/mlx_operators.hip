@@ -534,13 +534,14 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
         const int64_t piece = b / a.tiles, slot = ((b % a.tiles) << a.lpr) + lane, lo = piece * per, hi = lo + per;       // hi < n
         const uint32_t k = a.key[hi - 1], before = piece ? a.key[lo - 1] : 0xffffffffu;
         if (k >= (uint32_t)a.n_rows || before == k) continue;
-        // how many of the next pieces begin with this id: 64 are asked at a time
-        int64_t count = 0;
-        for (bool on = true; on;) {
-            const int64_t q = piece + 1 + count + (threadIdx.x & 63);
-            const uint64_t other = ~__ballot(q < a.pieces && a.key[q * per] == k);
-            on = other == 0;
-            count += on ? 64 : __ffsll((unsigned long long)other) - 1;
+        // how many of the next pieces begin with this id: the next 64 are asked, then 64 spread over what is left
+        int64_t count = 0, most = a.pieces - 1 - piece;
+        for (int64_t step = 1; most > count; step = (most - count + 63) / 64) {
+            const int64_t q = count + step * ((threadIdx.x & 63) + 1);
+            const uint64_t other = ~__ballot(q <= most && a.key[(q <= most ? piece + q : piece) * per] == k);
+            const int64_t same = other ? __ffsll((unsigned long long)other) - 1 : 64;
+            if (same < 64 && count + step * (same + 1) - 1 < most) most = count + step * (same + 1) - 1;
+            count += step * same;
         }
         if (count == 0) continue;
         const bool mine = slot < a.slots;

@@ -289,7 +289,7 @@ def test_gradient(ops, dtype, n, rows, width):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,width", [(40, 70), (4096, 24), (30000, 12)])
+@pytest.mark.parametrize("n,width", [(40, 70), (4096, 24), (30000, 12), (30000, 260), (2100, 520)])
 def test_gradient_of_one_id_and_of_none(ops, dtype, n, width):
     """Every entry the same id (one sum over all pieces), every entry absent, two ids that alternate, ids in descending order."""
     g = rng(n)
