@@ -533,7 +533,7 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
     for (int64_t b = blockIdx.x; b < (a.pieces - 1) * a.tiles; b += gridDim.x) {
         const int64_t piece = b / a.tiles, slot = ((b % a.tiles) << a.lpr) + lane, lo = piece * per, hi = lo + per;       // hi < n
         const uint32_t k = a.key[hi - 1], before = piece ? a.key[lo - 1] : 0xffffffffu;
-        if (k >= (uint32_t)a.n_rows || before == k) continue;
+        if (k >= (uint32_t)a.n_rows || before == k || a.key[hi] != k) continue;
         // how many of the next pieces begin with this id: the next 64 are asked, then 64 spread over what is left
         int64_t count = 0, most = a.pieces - 1 - piece;
         for (int64_t step = 1; most > count; step = (most - count + 63) / 64) {
@@ -548,7 +548,7 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
         float sum[E] = {};
         if (mine) {
             // pieces piece + 1 .. piece + count, and as number 0 the tail of `piece`
-#pragma unroll 8
+#pragma unroll 4
             for (int64_t q = group; q <= count; q += groups) {
                 const float *in = a.part + (((piece + q) * 2 + (q == 0)) * a.slots + slot) * E;
 #pragma unroll
@@ -683,7 +683,7 @@ __device__ __forceinline__ void put_loglik(float *logp, float *stats, int64_t t,
 {
     const double log_sum = log((double)a.s);
     logp[t] = a.m == -INFINITY && a.s == 0.0f ? -INFINITY : (float)(((double)value - (double)a.m) - log_sum);
-    stats[2 * t] = a.m;
+    stats[2 * t] = a.s != a.s ? a.s : a.m;                               // (a row of nothing but NaN has no maximum; -infinity would make its gradient 0)
     stats[2 * t + 1] = (float)log_sum;
 }
 template <class T, int LANES>

@@ -97,9 +97,14 @@ class HipOperators:
         return t.data_ptr()
 
     def _ids(self, t, what, n=None):
+        """(pointer, type) of a vector of ids."""
         if t.dim() != 1 or t.dtype not in self._id_types or (n is not None and t.shape[0] != n):
             raise ValueError("%s must be a vector of %sint32 or int64, not %s %s" % (what, "" if n is None else "%d " % n, tuple(t.shape), t.dtype))
-        return self._vector(t, what, t.shape[0], t.dtype), self._id_types[t.dtype]
+        if t.device != self._at:
+            raise ValueError("%s is on %s, these operators are on %s" % (what, t.device, self._at))
+        if not t.is_contiguous():
+            raise ValueError("%s must be contiguous" % what)
+        return t.data_ptr(), self._id_types[t.dtype]
 
     def _output(self, out, shape, dtype):
         """(tensor, pointer, ld) of a new matrix, or of the caller's."""

@@ -266,7 +266,8 @@ def check_gradient(got, grad_out, ids, rows, scale, before=None):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,rows,width", [(1, 1, 1), (1, 300, 64), (31, 5, 7), (32, 70000, 3), (33, 2, 130), (64, 1, 65), (1000, 17, 9), (2048, 256, 8), (2049, 257, 33), (5000, 65537, 1),
-                                          (700, 900, 1001), (20000, 3, 20), (100, 4, 9000), (17000, 40000, 64), (66000, 1000, 8)])
+                                          (700, 900, 1001), (20000, 3, 20), (100, 4, 9000), (17000, 40000, 64), (66000, 1000, 8),
+                                          (4096, 511, 4), (4097, 512, 4), (9000, 513, 6), (9000, 262143, 2), (5000, 262144, 3), (300000, 5000, 4), (262145, 300000, 1)])
 def test_gradient(ops, dtype, n, rows, width):
     g = rng(n + width)
     go = torch.randn(n, width, generator=g, device="cuda").to(dtype)
@@ -454,8 +455,9 @@ def test_loglik_masks_and_special_values(ops, dtype, classes):
     d = ops.token_loglik_gradient(y, t, stats, g4)
     assert d[0].isnan().all() and d[1].isnan().any() and not d[2:].any()
     # all rows NaN: still NaN
-    got, stats = ops.token_loglik(torch.full((1, classes), math.nan, device="cuda", dtype=dtype), t[:1])
-    assert got.isnan().all()
+    nan = torch.full((1, classes), math.nan, device="cuda", dtype=dtype)
+    got, stats = ops.token_loglik(nan, t[:1])
+    assert got.isnan().all() and ops.token_loglik_gradient(nan, t[:1], stats, g4[:1]).isnan().all()
 
 
 @gpu
@@ -719,6 +721,33 @@ def test_captured_step_replays(ops):
         got = [x.clone() for x in out]
         want = training_step(ops, table, head, ids, target, seq, ref)
         assert all(torch.equal(x, y) for x, y in zip(got, want)), k
+
+
+@gpu
+def test_two_captured_graphs_and_accumulation(ops):
+    """Gradients of two batches added to one table in two graphs, replayed in turn with eager work between: every replay adds what an eager
+    call adds, in the same bits."""
+    g = rng(13)
+    n, rows, width = 6000, 900, 72
+    batches = [(torch.randn(n, width, generator=g, device="cuda").to(torch.bfloat16), some_ids(g, n, rows, torch.int64)) for _ in range(2)]
+    acc = torch.zeros(rows, width, device="cuda")
+    for go, ids in batches:
+        ops.embedding_gradient(go, ids, rows, out=acc, accumulate=True)
+    graphs = []
+    for go, ids in batches:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.embedding_gradient(go, ids, rows, out=acc, accumulate=True)
+        graphs.append(graph)
+    acc.zero_()
+    want = torch.zeros_like(acc)
+    for k in range(5):
+        go, ids = batches[k % 2]
+        go.copy_(torch.randn(n, width, generator=g, device="cuda"))
+        graphs[k % 2].replay()
+        ops.embedding_gradient(go, ids, rows, out=want, accumulate=True)
+        torch.cuda.synchronize()
+        assert torch.equal(acc, want), k
 
 
 @gpu
