@@ -787,8 +787,6 @@ __global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, 
 // A sequence's sum is in 64 bits: it is a small difference of large terms' sums. Three shapes, by the sequences' average length and number:
 // 1 or 8 lanes a sequence where they are short, 256 lanes a sequence and a workgroup a pair, and for few long ones parts
 // of sequences, a workgroup each, whose sums the workgroups of the gradient's parts add up again.
-__device__ __forceinline__ double softplus(double h) { return fmax(h, 0.0) + log1p(exp(-fabs(h))); }
-__device__ __forceinline__ double logistic(double h) { return 1.0 / (1.0 + exp(-h)); }
 
 struct PrefArgs {
     const float *logp, *ref;
@@ -863,7 +861,8 @@ template <int LANES> __device__ __forceinline__ SeqSum join_sums(SeqSum s)
     }
     return s;
 }
-// what one pair comes to; its values are written where `writes`. Returns scale * weight * loss, and the gradients of the two sequences' tokens.
+// What one pair comes to: the gradients of the two sequences' tokens, and where `writes` its values are written and scale * weight * loss is returned.
+// e = exp(-|h|) serves all: log(1 + exp(h)) = max(h, 0) + log1p(e), and the logistic function of h and -h are 1 / (1 + e) and e / (1 + e) in some order.
 __device__ __forceinline__ double pair_of(const PrefArgs &a, int64_t p, const SeqSum (&s)[2], float (&g)[2], bool writes)
 {
     double ratio[2], part[2];
@@ -874,16 +873,16 @@ __device__ __forceinline__ double pair_of(const PrefArgs &a, int64_t p, const Se
     }
     const double h = (double)a.beta * (ratio[0] - ratio[1]) + (a.offset ? (double)a.offset[p] : 0.0), eps = (double)a.smoothing;
     const double w = (double)a.scale * (a.weight ? (double)a.weight[p] : 1.0);
-    // each term only where its factor is not 0: an infinite margin must not make 0 * infinity of the other one
-    const double loss = (eps < 1 ? (1 - eps) * softplus(-h) : 0.0) + (eps > 0 ? eps * softplus(h) : 0.0);
-    const double slope = w == 0 ? 0.0 : w * (double)a.beta * (eps * logistic(h) - (1 - eps) * logistic(-h));
+    const double e = exp(-fabs(h)), r = 1.0 / (1.0 + e), up = h >= 0 ? r : e * r, down = h >= 0 ? e * r : r;       // logistic of h and -h
+    const double slope = w == 0 ? 0.0 : w * (double)a.beta * (eps * up - (1 - eps) * down);
     g[0] = (float)(slope * part[0]);
     g[1] = (float)(-slope * part[1]);
-    if (writes) {
-        a.pair_loss[p] = (float)loss;
-        if (a.margin) a.margin[p] = (float)h;
-        if (a.ratio) { a.ratio[p] = (float)ratio[0]; a.ratio[a.pairs + p] = (float)ratio[1]; }
-    }
+    if (!writes) return 0;
+    // each term only where its factor is not 0: an infinite margin must not make 0 * infinity of the other one
+    const double l = log1p(e), loss = (eps < 1 ? (1 - eps) * (fmax(-h, 0.0) + l) : 0.0) + (eps > 0 ? eps * (fmax(h, 0.0) + l) : 0.0);
+    a.pair_loss[p] = (float)loss;
+    if (a.margin) a.margin[p] = (float)h;
+    if (a.ratio) { a.ratio[p] = (float)ratio[0]; a.ratio[a.pairs + p] = (float)ratio[1]; }
     return w == 0 ? 0.0 : w * loss;
 }
 // tokens before the first sequence and behind the last have no gradient
@@ -915,8 +914,7 @@ __global__ __launch_bounds__(256) void k_preference_short(PrefArgs a)
         if (!here) continue;
         const SeqSum both[2] = { side ? other : mine, side ? mine : other };
         float g[2];
-        const double x = pair_of(a, p, both, g, one);
-        if (one) loss += x;
+        loss += pair_of(a, p, both, g, one);
         if (a.grad) put_gradient<LANES>(a, r, lane, g[side]);
     }
     loss = wave_all(loss, [](double x, double y) { return x + y; });

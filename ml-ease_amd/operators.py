@@ -88,13 +88,13 @@ class HipOperators:
         return t.data_ptr(), t.stride(0)
 
     def _vector(self, t, what, n, dtype):
+        if t.dtype is dtype and t.shape == (n,) and t.device == self._at and t.is_contiguous():
+            return t.data_ptr()
         if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype:
             raise ValueError("%s must be a vector of %d %s, not %s %s" % (what, n, dtype, tuple(t.shape), t.dtype))
         if t.device != self._at:
             raise ValueError("%s is on %s, these operators are on %s" % (what, t.device, self._at))
-        if n > 1 and t.stride(0) != 1:
-            raise ValueError("%s must be contiguous" % what)
-        return t.data_ptr()
+        raise ValueError("%s must be contiguous" % what)
 
     def _ids(self, t, what, n=None):
         """(pointer, type) of a vector of ids."""
@@ -197,12 +197,15 @@ class HipOperators:
         mp = None if mask is None else self._vector(mask, "mask", n, torch.uint8 if mask.dtype == torch.uint8 else torch.bool)
         wp = None if weight is None else self._vector(weight, "weight", pairs, f32)
         fp = None if offset is None else self._vector(offset, "offset", pairs, f32)
-        # the few values of every pair in one block, the gradient in one of its own
-        few = torch.empty(4 * pairs + 1, dtype=f32, device=self._at)
-        ratio, pair_loss, margin, loss = few.split((2 * pairs, pairs, pairs, 1))
-        at = few.data_ptr()
+        # the workspace and the few values of every pair in one block, the gradient in one of its own
+        need = C.c_size_t()
+        self._ck(self.L.mlx_preference_loss_workspace(n, pairs, C.byref(need)))
+        kb = need.value
+        few = torch.empty((kb + 3) // 4 + 4 * pairs + 1, dtype=f32, device=self._at)
+        _, ratio, pair_loss, margin, loss = few.split(((kb + 3) // 4, 2 * pairs, pairs, pairs, 1))
+        kp = few.data_ptr()
+        at = kp + (kb + 3) // 4 * 4
         g = torch.empty(n, dtype=f32, device=self._at) if grad else None
-        keep, kp, kb = self._workspace(self.L.mlx_preference_loss_workspace, n, pairs)
         self._ck(self.L.mlx_preference_loss(self.device, self._stream(), lp, rp, n, qp, pairs, beta, smoothing, scale, bool(mean), mp, wp, fp, at + 16 * pairs,
                                             at + 8 * pairs, at + 12 * pairs, at, None if g is None else g.data_ptr(), kp, kb))
         return PreferenceResult(loss.view(()), pair_loss, margin, ratio, g)
