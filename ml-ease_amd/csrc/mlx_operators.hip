@@ -6,7 +6,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cfloat>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -38,7 +37,7 @@ template <class T> __device__ __forceinline__ T from_float(float x)
     return (T)x;
 }
 
-// NT: past the caches' usual replacement, for matrices that do not fit them and are read or written once (the entry points' rule: streams())
+// NT: past the caches' usual replacement (the entry points' rule: streams())
 template <bool NT, class T> __device__ __forceinline__ u32x4 load_raw(const T *p)
 {
     const auto *v = reinterpret_cast<const typename Chunk<T>::vec *>(p);
@@ -96,7 +95,9 @@ template <class T, class Op> __device__ __forceinline__ T wave_all(T x, Op op)
 }
 
 // ---------------------------------------------------------------------------------------------- lookup
-// 2^lpr lanes take a row, a lane every 2^lpr-th slot, 256 >> lpr rows a workgroup.
+// out[t] = scale table[ids[t]]: bound by memory, a read and a write of every row. 2^lpr lanes take a row, a lane every 2^lpr-th slot, 256 >> lpr
+// rows a workgroup, so that narrow rows fill the waves too. 16384 x 4096 bf16: 37 us, 5.1 TB/s of distinct rows read and rows written; the sweep's
+// 195300 x 8 f32: 4.5 us; 8 x 4096: 3.0 us, the launch's latency. (A slot a lane and more workgroups: 1 us slower.)
 template <class T, bool NT, bool NARROW>
 __global__ __launch_bounds__(256) void k_embedding_lookup(const T *__restrict__ table, int64_t n_rows, int64_t width, int64_t ldt, Ids ids, int64_t n, float scale,
                                                           T *__restrict__ out, int64_t ldo, int lpr, int64_t groups)
@@ -128,9 +129,12 @@ __global__ __launch_bounds__(256) void k_embedding_lookup(const T *__restrict__ 
 // ---------------------------------------------------------------------------------------------- gradient of the lookup
 // The entries are sorted by id (stable, so that equal ids keep ascending t), then sums run over the sorted list.
 //
-// Sort: least significant digit first, 9 bits a pass, absent entries (key n_rows) last. A workgroup owns a tile of consecutive entries
-// of the list; at most SORT_TILES tiles, so that every workgroup of a pass can add up the other tiles' counts by itself. A pass counts
-// the digits of the next one for the tile an entry goes to, so a pass is one launch. Lists of one tile sort in one launch, in LDS.
+// Sort: least significant digit first, 9 bits a pass (two passes up to 262143 rows), absent entries (key n_rows) last. A pass is two launches:
+// counts of the digits in every tile of the list, then every workgroup adds up the other tiles' counts by itself (hence SORT_TILES at most) and
+// moves its tile's entries. Bound by latency: 195300 entries of 100001 rows take 4 + 12 us a pass. Counting the next pass on the way, by atomics,
+// is slower (25 us), so are 1024 lanes a workgroup (14) and tiles of twice the size (13.5). Lists of up to ONE_TILE entries sort in one launch, in
+// LDS, by one workgroup: 5.5 us for 300 entries; 8000 entries would take 2 us longer that way than in tiles, 16000 20 us. While the sort keeps few
+// compute units busy, the other workgroups of its launches write the zeros of rows without an id (524 MB in 94 us).
 constexpr int DIGIT_BITS = 9, DIGITS = 1 << DIGIT_BITS, SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_TILES = 128;
 constexpr int64_t SORT_TILE = 2048, ONE_TILE = 4096;
 
@@ -194,8 +198,8 @@ __device__ __forceinline__ void fill_zero(G *grad, int64_t n_rows, int64_t width
 }
 template <class G> struct Zeros { G *grad; int64_t rows, width, ld; };      // the rows a launch writes along
 
-// Counts of the digits of a pass in every tile, [tiles][DIGITS] (workgroups 0 .. tiles - 1; the others write zeros). FIRST: entries come from
-// ids, else from key.
+// Counts of a pass's digits in every tile, [tiles][DIGITS] (workgroups 0 .. tiles - 1; the others write zeros). FIRST: entries come from ids, else
+// from key.
 template <class G, bool NT, bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void k_sort_count(Ids ids, int64_t n, int64_t n_rows, SortPlan plan, int shift, uint32_t *__restrict__ counts,
                                                              const uint32_t *__restrict__ key, Zeros<G> z)
@@ -362,6 +366,8 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_one_tile(Ids ids, int n, 
 // that goes on behind it) and of one that begins in it and goes on (its tail). Suffix sums over the heads, doubling their reach, give every
 // tail the rest of its id; ids that cross the borders of a workgroup's entries leave a sum before (part[0]) and behind (part[1]) the border
 // for k_piece_join. The order of the additions depends on n and width only.
+// Bound by memory for wide rows: 16384 x 4096 bf16 38 us for 123 MB read and 75 MB written in random rows, all loads of a group on their way at
+// once; by latency for narrow ones: 195300 x 8 f32 11 us. SEG 16 leaves fewer sums to join and 40 us, 15 us here; 4 leaves 14 us of joining (7 now).
 constexpr int SEG = 8;
 
 template <class T, class G, bool NT, bool NARROW> __device__ __forceinline__ void put_slot(G *row, const Slot<T> &at, const float (&sum)[Chunk<T>::N], float scale, bool add)
@@ -577,7 +583,7 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
 // The forward pass reads through the caches as usual, so that the backward pass finds in the memory-side cache what that holds of the logits;
 // that pass reads and writes past them (8192 x 32000 bf16, both passes: 174 us so, 212 us with the forward reads non-temporal too, 204 us with
 // the writes alone, 233 us with none).
-// Forward: one read of the row with the running maximum and sum of a softmax. A lane takes BATCH chunks at a time: their maximum first, one
+// Forward (57 to 66 us of the 174 for 315 MB): one read of the row with the running maximum and sum of a softmax. A lane takes BATCH chunks at a time: their maximum first, one
 // rescaling of the sum, then the exponentials. A maximum of -infinity (nothing but excluded classes so far) counts as 0 in the differences,
 // so that they stay -infinity and add 0. LANES lanes take a row; few long rows are cut into parts whose (max, sum) a second launch joins.
 // exp(t) = 2^(t log2 e) with log2 e in two parts: one part alone is off by 1.3e-8 of t in every term alike, 1e-7 of a typical row's sum, and
@@ -730,7 +736,8 @@ __global__ __launch_bounds__(64) void k_token_loglik_join(const T *__restrict__ 
     a = join_lanes<64>(a, nullptr);
     if (threadIdx.x == 0) put_loglik(logp, stats, t, a, to_float(logits[t * ld + y]));
 }
-// Backward: one read and one write of the row; the target's class as -expm1(log p), since 1 - p would lose the digits of a p near 1.
+// Backward: one read and one write of the row, bound by memory (115 to 118 us of the 174; 840 MB, some of the logits from the memory-side cache);
+// the target's class as -expm1(log p), since 1 - p would lose the digits of a p near 1.
 // A workgroup takes ROWS rows of LANES lanes, or a part of a row.
 template <class T, bool NT, int LANES>
 __global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, int64_t n, int64_t classes, int64_t ld, Ids target,
@@ -786,7 +793,9 @@ __global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, 
 // ---------------------------------------------------------------------------------------------- preference
 // A sequence's sum is in 64 bits: it is a small difference of large terms' sums. Three shapes, by the sequences' average length and number:
 // 1 or 8 lanes a sequence where they are short, 256 lanes a sequence and a workgroup a pair, and for few long ones parts
-// of sequences, a workgroup each, whose sums the workgroups of the gradient's parts add up again.
+// of sequences, a workgroup each, whose sums the workgroups of the gradient's parts add up again. Bound by latency (bounds, tokens, a sum across the
+// workgroup, the pair's exponential and logarithm in 64 bits, the gradient) at usual sizes: 256 pairs of 3900 tokens 9.6 us and 1.5 for the total,
+// 4 pairs of 125 tokens 5 us in one launch.
 
 struct PrefArgs {
     const float *logp, *ref;
@@ -1050,9 +1059,13 @@ int check_matrix(const char *who, const char *what, const void *p, int64_t rows,
     return MLX_OK;
 }
 
-// Matrices that are read or written once and do not fit the caches go past their usual replacement (non-temporal).
-constexpr int64_t CACHED = 32 << 20;
-bool streams(int64_t rows, int64_t width, int64_t es) { return rows * width * es > CACHED; }
+// Matrices go past the caches' usual replacement (non-temporal) where what a call writes, or reads once and writes, is more than the memory-side
+// cache holds: the next reader would not find it there, and its write-back would run beside the next kernel. Measured, non-temporal / usual, alone
+// and with the row norms of the result taken right behind it: 8192 x 32000 bf16 loglik forward and backward 175 / 234, 299 / 348 us; 777 x 50021
+// f32 82 / 107, 120 / 123; gradient of 16384 x 4096 bf16 into 64000 rows 141 / 159, 249 / 278. Below the limit it is the other way about once there
+// is a reader: lookup of 16384 x 4096 bf16 (134 MB) 34 / 37 alone, 73 / 64 with the norms; logits of 64 MB even.
+constexpr int64_t MEMORY_SIDE_CACHE = 256ll << 20;
+bool streams(int64_t rows, int64_t width, int64_t bytes) { return rows * width > MEMORY_SIDE_CACHE / bytes; }
 
 struct GradientPlan { SortPlan sort; int lpr; int64_t slots, tiles, pieces; size_t key, counts, part, bytes; };
 GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
@@ -1326,7 +1339,7 @@ int mlx_token_loglik_gradient(int32_t device, void *stream, int32_t type, const 
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
         const LoglikPlan plan = loglik_plan(es, n_tokens, n_classes);
-        return by_flag(plan.grad_lanes == 256 && streams(n_tokens, n_classes, es), [&](auto nt) {
+        return by_flag(plan.grad_lanes == 256 && streams(n_tokens, n_classes, 2 * es), [&](auto nt) {
             return by_lanes(plan.grad_lanes, [&](auto l) {
                 constexpr int LANES = decltype(l)::value;
                 hipLaunchKernelGGL((k_token_loglik_gradient<T, nt.value, LANES>), dim3(grid_of(ceil_div(n_tokens * plan.grad_parts, 256 / LANES))), dim3(256), 0, (hipStream_t)stream,
