@@ -600,11 +600,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));       // fmaxf would quiet both operands first, an operation each
     return d;
 }
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b)
-{
-    const float m = fmaxf(a.m, b.m), r = finite_max(m);
-    return { m, a.s * exp_of(a.m - r) + b.s * exp_of(b.m - r) };
-}
 template <int N> __device__ __forceinline__ void add_values(MaxSum &a, const float (&f)[N])
 {
     float m = a.m;
@@ -618,41 +613,47 @@ template <int N> __device__ __forceinline__ void add_values(MaxSum &a, const flo
     for (int i = 0; i < N; i++) more[i & 3] += exp_of(f[i] - r);
     a = { m, s + ((more[0] + more[1]) + (more[2] + more[3])) };
 }
-// Chunks c0 .. c1 of a row and its last elements (where `rest`) by LANES lanes. The next BATCH chunks are on their way while these are added:
-// two sets of registers, and loads that are always made (behind the end the last chunk again, not looked at), since a wait behind loads that
-// some lanes may have skipped is a wait for all of them.
-template <class T, int LANES> __device__ __forceinline__ MaxSum row_part(const T *x, int64_t c0, int64_t c1, int64_t classes, bool rest, int lane)
+// Chunks c0 .. c1 of a row and its last elements (where `rest`) by LANES lanes, without class y. The next BATCH chunks are on their way while
+// these are added: two sets of registers, and loads that are always made (behind the end the last chunk again, not looked at), since a wait
+// behind loads that some lanes may have skipped is a wait for all of them.
+template <class T, int LANES> __device__ __forceinline__ MaxSum row_part(const T *x, int c0, int c1, int classes, int y, bool rest, int lane)
 {
     constexpr int E = Chunk<T>::N, B = LANES == 1024 ? BATCH / 2 : BATCH, STEP = B * LANES;       // (1024 lanes have 128 registers each)
     MaxSum a = { -INFINITY, 0.0f };
     typedef u32x4 Set[B];
-    auto fetch = [&](Set &v, int64_t base) {
+    auto fetch = [&](Set &v, int base) {
 #pragma unroll
         for (int i = 0; i < B; i++) {
-            const int64_t c = base + i * LANES + lane;
-            v[i] = load_raw<false>(x + (c < c1 ? c : c1 - 1) * E);
+            const int c = base + i * LANES + lane;
+            v[i] = load_raw<false>(x + (int64_t)(c < c1 ? c : c1 - 1) * E);
         }
     };
-    auto add = [&](Set &v, int64_t base) {
+    auto values = [&](u32x4 raw, int c, float *f) {
+        unpack<T>(raw, f);
+        if (c == y / E)
+#pragma unroll
+            for (int e = 0; e < E; e++) f[e] = e == y % E ? -INFINITY : f[e];
+    };
+    auto add = [&](Set &v, int base) {
         if (base + STEP > c1) {                                          // the row's last chunks: one at a time, none for lanes behind the end
 #pragma unroll
             for (int i = 0; i < B; i++)
                 if (base + i * LANES + lane < c1) {
                     float f[E];
-                    unpack<T>(v[i], f);
+                    values(v[i], base + i * LANES + lane, f);
                     add_values(a, f);
                 }
             return;
         }
         float f[B * E];
 #pragma unroll
-        for (int i = 0; i < B; i++) unpack<T>(v[i], f + i * E);
+        for (int i = 0; i < B; i++) values(v[i], base + i * LANES + lane, f + i * E);
         add_values(a, f);
     };
     if (c0 < c1) {
         Set p, q;
         fetch(p, c0);
-        for (int64_t base = c0;; base += 2 * STEP) {
+        for (int base = c0;; base += 2 * STEP) {
             if (base + STEP >= c1) { add(p, base); break; }
             fetch(q, base + STEP);
             __builtin_amdgcn_sched_barrier(0);
@@ -663,78 +664,125 @@ template <class T, int LANES> __device__ __forceinline__ MaxSum row_part(const T
             add(q, base + STEP);
         }
     }
-    const int64_t j = classes / E * E + lane;
-    if (rest && j < classes) {
+    const int j = classes / E * E + lane;
+    if (rest && lane < classes % E && j != y) {
         const float f[1] = { to_float(x[j]) };
         add_values(a, f);
     }
     return a;
 }
-template <int LANES> __device__ __forceinline__ MaxSum join_lanes(MaxSum a, MaxSum *ws)
+// Lanes' sums come together in 64 bits, and the target's class is added last: where it is the likely one the others are a small addition to its 1,
+// whose digits a 32-bit sum would lose, and log p with them.
+struct RowSum { double s; float m; };
+template <int LANES> __device__ __forceinline__ RowSum join_lanes(MaxSum a, RowSum *ws)
 {
+    constexpr int WIDE = LANES < 64 ? LANES : 64;
+    RowSum all;
+    all.m = a.m;
 #pragma unroll
-    for (int m = LANES < 64 ? LANES / 2 : 32; m; m >>= 1) a = join(a, { __shfl_xor(a.m, m), __shfl_xor(a.s, m) });
+    for (int m = WIDE / 2; m; m >>= 1) all.m = fmaxf(all.m, __shfl_xor(all.m, m));
+    all.s = (double)a.s * (double)exp_of(a.m - finite_max(all.m));
+#pragma unroll
+    for (int m = WIDE / 2; m; m >>= 1) all.s += __shfl_xor(all.s, m);
     if constexpr (LANES > 64) {
-        if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = a;
+        if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = all;
         __syncthreads();
-        a = ws[0];
+        all.m = -INFINITY;
 #pragma unroll
-        for (int w = 1; w < LANES / 64; w++) a = join(a, ws[w]);
+        for (int w = 0; w < LANES / 64; w++) all.m = fmaxf(all.m, ws[w].m);
+        all.s = 0;
+#pragma unroll
+        for (int w = 0; w < LANES / 64; w++) all.s += ws[w].s * (double)exp_of(ws[w].m - finite_max(all.m));
         __syncthreads();
     }
-    return a;
+    return all;
 }
-// the last steps in 64 bits: a pair's margin adds up small differences of many of these
-__device__ __forceinline__ void put_loglik(float *logp, float *stats, int64_t t, MaxSum a, float value)
+// `others`: all classes but the target's, whose logit is `value`. The last steps are in 64 bits: a pair's margin adds up small differences of many.
+// v_exp_f32 gives 3.4e-9 of its value too little on average (over 4 million arguments in each of [-1, 0] .. [-30, 0]: 3.1e-9 .. 3.4e-9; single results are
+// off by 2.6e-8 on average, 8.4e-8 at most), which is put back: answers of a hundred thousand tokens add that up.
+constexpr double EXP_MEAN_LOSS = 3.4e-9;
+// log(1 + x) for x >= 0, to 1e-11 of its value: 1 + x = 2^e f with f in [0.75, 1.5), and log f = 2 artanh z with z = (f - 1) / (f + 1), |z| <= 0.2, by its
+// series; where e = 0, f - 1 is x with all its digits. (The library's log1p and log, once a row, made rows of 100 to 1000 classes 30 % slower.)
+__device__ __forceinline__ double log_1_plus(double x)
 {
-    const double log_sum = log((double)a.s);
-    logp[t] = a.m == -INFINITY && a.s == 0.0f ? -INFINITY : (float)(((double)value - (double)a.m) - log_sum);
-    stats[2 * t] = a.s != a.s ? a.s : a.m;                               // (a row of nothing but NaN has no maximum; -infinity would make its gradient 0)
+    const double one_x = 1.0 + x;
+    double f = __builtin_amdgcn_frexp_mant(one_x);                       // [0.5, 1)
+    int e = __builtin_amdgcn_frexp_exp(one_x);
+    const bool low = f < 0.75;
+    f = low ? f + f : f;
+    e = low ? e - 1 : e;
+    const double num = e == 0 ? x : f - 1.0, den = num + 2.0;
+    double r = (double)__builtin_amdgcn_rcpf((float)den);                // to 1e-7, and one step of Newton's
+    r = r * __builtin_fma(-den, r, 2.0);
+    const double z = num * r, w = z * z;
+    double p = 1.0 / 13;
+    p = __builtin_fma(p, w, 1.0 / 11);
+    p = __builtin_fma(p, w, 1.0 / 9);
+    p = __builtin_fma(p, w, 1.0 / 7);
+    p = __builtin_fma(p, w, 1.0 / 5);
+    p = __builtin_fma(p, w, 1.0 / 3);
+    return __builtin_fma((double)e, 0.693147180559945309417, 2.0 * __builtin_fma(z * w, p, z));
+}
+__device__ __forceinline__ void put_loglik(float *logp, float *stats, int64_t t, RowSum others, float value)
+{
+    const float m = fmaxf(others.m, value), r = finite_max(m);
+    const double rest = others.s * (1.0 + EXP_MEAN_LOSS) * (double)exp_of(others.m - r), s = rest + (double)exp_of(value - r);
+    const double log_sum = m == -INFINITY ? (double)-INFINITY : log_1_plus(value == m ? rest : s - 1.0);
+    logp[t] = m == -INFINITY && s == 0 ? -INFINITY : (float)(((double)value - (double)m) - log_sum);
+    stats[2 * t] = s != s ? (float)s : m;                                // (a row of nothing but NaN has no maximum; -infinity would make its gradient 0)
     stats[2 * t + 1] = (float)log_sum;
 }
+__device__ __forceinline__ void put_absent(float *logp, float *stats, int64_t t) { logp[t] = stats[2 * t] = stats[2 * t + 1] = 0.0f; }
 template <class T, int LANES>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_token_loglik(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target,
-                                                      float *__restrict__ logp, float *__restrict__ stats)
+                                                                            float *__restrict__ logp, float *__restrict__ stats)
 {
     constexpr int ROWS = LANES < 256 ? 256 / LANES : 1;
-    __shared__ MaxSum ws[LANES < 64 ? 1 : LANES / 64];
+    __shared__ RowSum ws[LANES < 64 ? 1 : LANES / 64];
     const int lane = threadIdx.x & (LANES - 1);
     for (int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; t < n; t += (int64_t)gridDim.x * ROWS) {
-        const int64_t y = id_at(target, t, classes);
+        const int y = (int)id_at(target, t, classes);
         if (y < 0) {
-            if (lane == 0) { logp[t] = 0.0f; stats[2 * t] = 0.0f; stats[2 * t + 1] = 0.0f; }
+            if (lane == 0) put_absent(logp, stats, t);
             continue;
         }
         const T *x = logits + t * ld;
-        const MaxSum a = join_lanes<LANES>(row_part<T, LANES>(x, 0, classes / Chunk<T>::N, classes, true, lane), ws);
-        if (lane == 0) put_loglik(logp, stats, t, a, to_float(x[y]));
+        const float value = to_float(x[y]);
+        const RowSum others = join_lanes<LANES>(row_part<T, LANES>(x, 0, (int)(classes / Chunk<T>::N), (int)classes, y, true, lane), ws);
+        if (lane == 0) put_loglik(logp, stats, t, others, value);
     }
 }
 // parts of rows, [n][parts] of workspace; parts <= 64
 template <class T>
 __global__ __launch_bounds__(256) void k_token_loglik_parts(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target, int parts,
-                                                            MaxSum *__restrict__ out)
+                                                            RowSum *__restrict__ out)
 {
-    __shared__ MaxSum ws[4];
-    const int64_t t = blockIdx.x / parts, part = blockIdx.x % parts;
-    if (id_at(target, t, classes) < 0) return;
-    const int64_t chunks = classes / Chunk<T>::N, step = (chunks + parts - 1) / parts, c0 = part * step < chunks ? part * step : chunks, c1 = c0 + step < chunks ? c0 + step : chunks;
-    const MaxSum a = join_lanes<256>(row_part<T, 256>(logits + t * ld, c0, c1, classes, part == parts - 1, threadIdx.x), ws);
+    __shared__ RowSum ws[4];
+    const int64_t t = blockIdx.x / parts;
+    const int part = blockIdx.x % parts, y = (int)id_at(target, t, classes);
+    if (y < 0) return;
+    const int chunks = (int)(classes / Chunk<T>::N), step = (chunks + parts - 1) / parts, c0 = part * step < chunks ? part * step : chunks, c1 = c0 + step < chunks ? c0 + step : chunks;
+    const RowSum a = join_lanes<256>(row_part<T, 256>(logits + t * ld, c0, c1, (int)classes, y, part == parts - 1, threadIdx.x), ws);
     if (threadIdx.x == 0) out[blockIdx.x] = a;
 }
 template <class T>
 __global__ __launch_bounds__(64) void k_token_loglik_join(const T *__restrict__ logits, int64_t n, int64_t classes, int64_t ld, Ids target, int parts,
-                                                          const MaxSum *__restrict__ in, float *__restrict__ logp, float *__restrict__ stats)
+                                                          const RowSum *__restrict__ in, float *__restrict__ logp, float *__restrict__ stats)
 {
     const int64_t t = blockIdx.x, y = id_at(target, t, classes);
     if (y < 0) {
-        if (threadIdx.x == 0) { logp[t] = 0.0f; stats[2 * t] = 0.0f; stats[2 * t + 1] = 0.0f; }
+        if (threadIdx.x == 0) put_absent(logp, stats, t);
         return;
     }
-    MaxSum a = { -INFINITY, 0.0f };
+    RowSum a = { 0, -INFINITY };
     if ((int)threadIdx.x < parts) a = in[t * parts + threadIdx.x];
-    a = join_lanes<64>(a, nullptr);
-    if (threadIdx.x == 0) put_loglik(logp, stats, t, a, to_float(logits[t * ld + y]));
+    RowSum all = a;
+#pragma unroll
+    for (int m = 32; m; m >>= 1) all.m = fmaxf(all.m, __shfl_xor(all.m, m));
+    all.s = a.s * (double)exp_of(a.m - finite_max(all.m));
+#pragma unroll
+    for (int m = 32; m; m >>= 1) all.s += __shfl_xor(all.s, m);
+    if (threadIdx.x == 0) put_loglik(logp, stats, t, all, to_float(logits[t * ld + y]));
 }
 // Backward: one read and one write of the row, bound by memory (115 to 118 us of the 174; 840 MB, some of the logits from the memory-side cache);
 // the target's class as -expm1(log p), since 1 - p would lose the digits of a p near 1.
@@ -1106,7 +1154,7 @@ LoglikPlan loglik_plan(int64_t es, int64_t n, int64_t classes)
     p.grad_parts = n >= 512 || n == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({ 64, ceil_div(512, n), chunks / (256 * BATCH) }));
     p.parts = classes > LONG_ROW ? p.grad_parts : 1;
     if (n <= 512 && p.grad_parts > 1) p.lanes = 1024;
-    p.bytes = p.parts > 1 ? (size_t)(n * p.parts) * sizeof(MaxSum) : 0;
+    p.bytes = p.parts > 1 ? (size_t)(n * p.parts) * sizeof(RowSum) : 0;
     return p;
 }
 template <class F> int by_lanes(int lanes, F &&f)
@@ -1298,9 +1346,9 @@ int mlx_token_loglik(int32_t device, void *stream, int32_t type, const void *log
         const Ids y = { target, id_type == MLX_I64 };
         if (plan.parts > 1) {
             hipLaunchKernelGGL((k_token_loglik_parts<T>), dim3((unsigned)(n_tokens * plan.parts)), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
-                               (MaxSum *)workspace);
+                               (RowSum *)workspace);
             hipLaunchKernelGGL((k_token_loglik_join<T>), dim3((unsigned)n_tokens), dim3(64), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
-                               (const MaxSum *)workspace, logp, stats);
+                               (const RowSum *)workspace, logp, stats);
             return 0;
         }
         if (plan.lanes == 1024) {

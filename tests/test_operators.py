@@ -461,6 +461,34 @@ def test_loglik_masks_and_special_values(ops, dtype, classes):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [2, 4, 100, 3001, 32000, 200001])
+def test_loglik_of_likely_targets(ops, dtype, classes):
+    """Targets nearly certain: log p = -log(1 + R) keeps its digits, R being the others' sum. R is off by what any sum of exponentials is (as in
+    exact_loglik, relative to the others' maximum) and by its rescaling to the target's logit."""
+    g = rng(classes)
+    x = torch.randn(12, classes, generator=g, device="cuda")
+    target = torch.randint(0, classes, (12,), generator=g, device="cuda")
+    rows = torch.arange(12, device="cuda")
+    x[rows, target] = torch.linspace(4, 40, 12, device="cuda")
+    x = x.to(dtype)
+    v, at = x.double(), target[:, None]
+    value = v.gather(1, at)
+    others = v.scatter(1, at, -math.inf)
+    top = others.amax(1, keepdim=True)
+    e = (others - top).exp()
+    mean_t = torch.where(e > 0, e * (others - top).abs(), 0.0).sum(1) / e.sum(1)
+    R = (e.sum(1, keepdim=True) * (top - value).exp())[:, 0]
+    want = -R.log1p()
+    err = U * (3 * mean_t + 2 + 2 * math.ceil(classes / 64) + 64 + 3 * (top - value).abs()[:, 0] + 3)
+    got, stats = ops.token_loglik(x, target)
+    within(got, want, R / (1 + R) * err * 1.01 + half_step(want, torch.float32) * (1 + 1e-6) + 2.0 ** -126)
+    d = ops.token_loglik_gradient(x, target, stats, torch.ones(12, device="cuda")).double().gather(1, at)[:, 0]
+    p_not = -torch.expm1(want)
+    within(d, p_not, p_not * (err * 1.01 + 8 * U) + half_step(p_not, dtype) * (1 + 1e-6) + 2.0 ** -126)
+
+
+@gpu
 def test_loglik_of_nothing(ops):
     x = torch.zeros(0, 9, device="cuda")
     logp, stats = ops.token_loglik(x, torch.empty(0, dtype=torch.int64, device="cuda"))
