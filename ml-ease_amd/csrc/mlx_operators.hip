@@ -177,16 +177,31 @@ __device__ __forceinline__ uint32_t key_at(Ids ids, int64_t t, int64_t n_rows)
     return (uint32_t)(id < 0 ? n_rows : id);
 }
 
-// rows [0, n_rows) of grad to zero by workgroups part, part + parts, ... ; the whole matrix as one row where it is dense
+// The rows of grad that a launch writes along: zeros by workgroups part, part + parts, ... . With `owner` those without an id only, a wave a row: every entry has put its number into its row's place of owner, so a row has an id if the entry named there is one of it;
+// places of other rows were never written and may hold anything. Without, the whole matrix is one row where it is dense.
+template <class G> struct Zeros { G *grad; int64_t rows, width, ld; const uint32_t *owner; Ids ids; int64_t n, first; };
 template <class G, bool NT>
-__device__ __forceinline__ void fill_zero(G *grad, int64_t n_rows, int64_t width, int64_t ld, int64_t part, int64_t parts)
+__device__ __forceinline__ void fill_zero(const Zeros<G> &z, int64_t part, int64_t parts)
 {
     constexpr int E = Chunk<G>::N;
     const float zero[E] = {};
-    if (ld == width) { width *= n_rows; n_rows = 1; }
+    int64_t n_rows = z.rows, width = z.width;
+    if (z.owner) {
+        const int64_t chunks = width / E;
+        const int lane = threadIdx.x & 63;
+        for (int64_t r = part * SORT_WAVES + (threadIdx.x >> 6); r < n_rows; r += parts * SORT_WAVES) {
+            const uint32_t entry = z.owner[z.first + r];
+            if (entry < z.n && id_at(z.ids, entry, INT64_MAX) == z.first + r) continue;
+            G *row = z.grad + r * z.ld;
+            for (int64_t s = lane; s < chunks; s += 64) store_chunk<NT>(row + s * E, zero);
+            if (lane < width % E) row[chunks * E + lane] = from_float<G>(0.0f);
+        }
+        return;
+    }
+    if (z.ld == width) { width *= n_rows; n_rows = 1; }
     const int64_t chunks = width / E, slots = chunks + width % E, step = 4 * SORT_THREADS, cuts = (slots + step - 1) / step;
     for (int64_t b = part; b < cuts * n_rows; b += parts) {
-        G *row = grad + (b / cuts) * ld;
+        G *row = z.grad + (b / cuts) * z.ld;
         const int64_t first = (b % cuts) * step + threadIdx.x;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -196,24 +211,27 @@ __device__ __forceinline__ void fill_zero(G *grad, int64_t n_rows, int64_t width
         }
     }
 }
-template <class G> struct Zeros { G *grad; int64_t rows, width, ld; };      // the rows a launch writes along
 
 // Counts of a pass's digits in every tile, [tiles][DIGITS] (workgroups 0 .. tiles - 1; the others write zeros). FIRST: entries come from ids, else
 // from key.
 template <class G, bool NT, bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void k_sort_count(Ids ids, int64_t n, int64_t n_rows, SortPlan plan, int shift, uint32_t *__restrict__ counts,
-                                                             const uint32_t *__restrict__ key, Zeros<G> z)
+                                                             const uint32_t *__restrict__ key, uint32_t *owner, Zeros<G> z)
 {
     __shared__ uint32_t cnt[DIGITS];
     if ((int)blockIdx.x >= plan.tiles) {
-        fill_zero<G, NT>(z.grad, z.rows, z.width, z.ld, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
+        fill_zero<G, NT>(z, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
         return;
     }
     cnt[threadIdx.x] = 0;
     __syncthreads();
     const int64_t lo = (int64_t)blockIdx.x * plan.tile, hi = lo + plan.tile < n ? lo + plan.tile : n;
 #pragma unroll 4
-    for (int64_t t = lo + threadIdx.x; t < hi; t += SORT_THREADS) atomicAdd(&cnt[((FIRST ? key_at(ids, t, n_rows) : key[t]) >> shift) & (DIGITS - 1)], 1u);
+    for (int64_t t = lo + threadIdx.x; t < hi; t += SORT_THREADS) {
+        const uint32_t k = FIRST ? key_at(ids, t, n_rows) : key[t];
+        atomicAdd(&cnt[(k >> shift) & (DIGITS - 1)], 1u);
+        if (FIRST && owner && k < (uint32_t)n_rows) owner[k] = (uint32_t)t;      // (of several entries any)
+    }
     __syncthreads();
     counts[(int64_t)blockIdx.x * DIGITS + threadIdx.x] = cnt[threadIdx.x];
 }
@@ -228,7 +246,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_move(Ids ids, int64_t n, 
     constexpr int AHEAD = 4, COLUMN = 32;
     __shared__ uint32_t at[SORT_WAVES][DIGITS], waves[SORT_WAVES];
     if ((int)blockIdx.x >= plan.tiles) {
-        fill_zero<G, NT>(z.grad, z.rows, z.width, z.ld, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
+        fill_zero<G, NT>(z, blockIdx.x - plan.tiles, gridDim.x - plan.tiles);
         return;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -304,7 +322,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_one_tile(Ids ids, int n, 
     __shared__ uint32_t at[SORT_WAVES][DIGITS], waves[SORT_WAVES], lkey[ONE_TILE];
     __shared__ uint16_t lpos[ONE_TILE];
     if (blockIdx.x > 0) {
-        fill_zero<G, NT>(z.grad, z.rows, z.width, z.ld, blockIdx.x - 1, gridDim.x - 1);
+        fill_zero<G, NT>(z, blockIdx.x - 1, gridDim.x - 1);
         return;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -583,8 +601,8 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
 // The forward pass reads through the caches as usual, so that the backward pass finds in the memory-side cache what that holds of the logits;
 // that pass reads and writes past them (8192 x 32000 bf16, both passes: 174 us so, 212 us with the forward reads non-temporal too, 204 us with
 // the writes alone, 233 us with none).
-// Forward (57 to 66 us of the 174 for 315 MB): one read of the row with the running maximum and sum of a softmax. A lane takes BATCH chunks at a time: their maximum first, one
-// rescaling of the sum, then the exponentials. A maximum of -infinity (nothing but excluded classes so far) counts as 0 in the differences,
+// Forward (57 to 66 us of the 174 for 315 MB): one read of the row with the running maximum and sum of a softmax. A lane takes BATCH chunks at a
+// time: their maximum first, one rescaling of the sum, then the exponentials. A maximum of -infinity (nothing but excluded classes so far) counts as 0 in the differences,
 // so that they stay -infinity and add 0. LANES lanes take a row; few long rows are cut into parts whose (max, sum) a second launch joins.
 // exp(t) = 2^(t log2 e) with log2 e in two parts: one part alone is off by 1.3e-8 of t in every term alike, 1e-7 of a typical row's sum, and
 // a pair's margin adds that up over hundreds of tokens (measured: margins of 512-token pairs off by 4e-6, with both parts by 5e-7).
@@ -1115,7 +1133,11 @@ int check_matrix(const char *who, const char *what, const void *p, int64_t rows,
 constexpr int64_t MEMORY_SIDE_CACHE = 256ll << 20;
 bool streams(int64_t rows, int64_t width, int64_t bytes) { return rows * width > MEMORY_SIDE_CACHE / bytes; }
 
-struct GradientPlan { SortPlan sort; int lpr; int64_t slots, tiles, pieces; size_t key, counts, part, bytes; };
+// Rows with an id are spared the zeros where that may be much of the table and a row is long enough to be asked about: 65536 entries of 4096 bf16 in
+// 32000 rows 221 us (frequent ids) and 211 (uniform) instead of 240 and 256, 16384 entries in 32000 rows 109 and 103 instead of 111 and 113; with a
+// quarter of the rows' number in entries 144 and 143 instead of 142 and 153, with an eighth 126 and 127 instead of 121 and 128.
+constexpr int64_t OWNER_WIDTH = 2048;
+struct GradientPlan { SortPlan sort; int lpr; bool owner; int64_t slots, tiles, pieces; size_t key, counts, owners, part, bytes; };
 GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
 {
     GradientPlan g;
@@ -1132,8 +1154,10 @@ GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
     auto round = [](size_t b) { return (b + 255) / 256 * 256; };
     g.key = round((size_t)n * 4);
     g.counts = n <= ONE_TILE ? 0 : round((size_t)g.sort.tiles * DIGITS * 4);
+    g.owner = n > ONE_TILE && width >= OWNER_WIDTH && n >= n_rows / 2;
+    g.owners = g.owner ? round((size_t)n_rows * 4) : 0;
     g.part = g.pieces > 1 ? round((size_t)g.pieces * 2 * (size_t)g.slots * (size_t)E * 4) : 0;
-    g.bytes = 4 * g.key + g.counts + g.part;
+    g.bytes = 4 * g.key + g.counts + g.owners + g.part;
     return g;
 }
 
@@ -1165,7 +1189,8 @@ template <class F> int by_lanes(int lanes, F &&f)
 
 // Short sequences (4, 64 tokens on average) have 1, 8 lanes each, others 256 (of one million pairs of one token 8 lanes each take 249 us: the pair's
 // logarithm and exponentials in 64 bits are every lane's work); where that makes fewer than 256 workgroups of sequences of
-// more than 8192 tokens on average, these are cut into parts of 4096 or more, 64 at most and 1024 workgroups in all.
+// more than 8192 tokens on average, these are cut into parts of 4096 or more, 64 at most and 1024 workgroups in all. (Lengths are on the device: one
+// sequence far above the average takes the time of its tokens by the lanes that the average gave it.)
 struct PrefPlan { int lanes, parts; int64_t groups; size_t sums, bytes; };
 PrefPlan preference_plan(int64_t n, int64_t pairs)
 {
@@ -1253,7 +1278,8 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
     char *w = (char *)workspace;
     uint32_t *key[2] = { (uint32_t *)w, (uint32_t *)(w + plan.key) }, *pos[2] = { (uint32_t *)(w + 2 * plan.key), (uint32_t *)(w + 3 * plan.key) };
     uint32_t *counts = (uint32_t *)(w + 4 * plan.key);
-    float *part = (float *)(w + 4 * plan.key + plan.counts);
+    uint32_t *owner = plan.owner && !accumulate ? (uint32_t *)(w + 4 * plan.key + plan.counts) : nullptr;
+    float *part = (float *)(w + 4 * plan.key + plan.counts + plan.owners);
     auto with = [&](auto t, auto g, auto nt, auto narrow) {
         typedef decltype(t) T;
         typedef decltype(g) G;
@@ -1266,9 +1292,11 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
         int share = 0;
         unsigned blocks = 0;
         auto zeros = [&]() {
-            const int64_t end = accumulate ? 0 : n_rows * ++share / shares, rows = end - row;
-            const Zeros<G> z = { out + row * ld_grad, rows, width, ld_grad };
-            blocks = rows > 0 ? (unsigned)std::min<int64_t>(2048, ceil_div(rows * width, 4 * SORT_THREADS * Chunk<G>::N)) : 0;
+            // (the entries' numbers are there from the second launch on)
+            const int64_t end = accumulate ? 0 : owner ? n_rows * share / (shares - 1) : n_rows * (share + 1) / shares, rows = end - row;
+            share++;
+            const Zeros<G> z = { out + row * ld_grad, rows, width, ld_grad, owner, id, n_ids, row };
+            blocks = rows > 0 ? (unsigned)std::min<int64_t>(2048, owner ? ceil_div(rows, SORT_WAVES) : ceil_div(rows * width, 4 * SORT_THREADS * Chunk<G>::N)) : 0;
             row = end;
             return z;
         };
@@ -1283,7 +1311,7 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
                     const int shift = pass * DIGIT_BITS;
                     Zeros<G> z = zeros();
                     hipLaunchKernelGGL((k_sort_count<G, NT, FIRST>), dim3(plan.sort.tiles + blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, shift, counts,
-                                       key[cur], z);
+                                       key[cur], owner, z);
                     z = zeros();
                     const int to = FIRST ? 0 : cur ^ 1;
                     hipLaunchKernelGGL((k_sort_move<G, NT, FIRST>), dim3(plan.sort.tiles + blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, shift, counts,

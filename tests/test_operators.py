@@ -267,7 +267,8 @@ def check_gradient(got, grad_out, ids, rows, scale, before=None):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,rows,width", [(1, 1, 1), (1, 300, 64), (31, 5, 7), (32, 70000, 3), (33, 2, 130), (64, 1, 65), (1000, 17, 9), (2048, 256, 8), (2049, 257, 33), (5000, 65537, 1),
                                           (700, 900, 1001), (20000, 3, 20), (100, 4, 9000), (17000, 40000, 64), (66000, 1000, 8),
-                                          (4096, 511, 4), (4097, 512, 4), (9000, 513, 6), (9000, 262143, 2), (5000, 262144, 3), (300000, 5000, 4), (262145, 300000, 1)])
+                                          (4096, 511, 4), (4097, 512, 4), (9000, 513, 6), (9000, 262143, 2), (5000, 262144, 3), (300000, 5000, 4), (262145, 300000, 1),
+                                          (5000, 900, 2051), (4500, 9000, 2048), (4500, 9001, 2055), (4097, 8194, 2300)])
 def test_gradient(ops, dtype, n, rows, width):
     g = rng(n + width)
     go = torch.randn(n, width, generator=g, device="cuda").to(dtype)
@@ -312,6 +313,11 @@ def test_gradient_strides_and_alignment(ops, dtype):
         out = ops.embedding_gradient(go, ids, 30, out=into[:, first + 1:first + 78])
         check_gradient(out, go, ids, 30, 1.0)
         assert (into[:, :first + 1] == 9).all() and (into[:, first + 78:] == 9).all()
+    wide = torch.randn(5000, 2100, generator=g, device="cuda").to(dtype)        # many entries of wide rows: rows with an id are spared the zeros
+    many = some_ids(g, 5000, 3000, torch.int64)
+    into = torch.full((3000, 2110), 9.0, device="cuda", dtype=dtype)
+    check_gradient(ops.embedding_gradient(wide[:, 1:2090], many, 3000, out=into[:, 3:2092]), wide[:, 1:2090], many, 3000, 1.0)
+    assert (into[:, :3] == 9).all() and (into[:, 2092:] == 9).all()
     same = whole[:1, :40].expand(200, 40)                                        # the gradient of a broadcast: one row for all entries
     check_gradient(ops.embedding_gradient(same, ids, 30), same, ids, 30, 1.0)
 
