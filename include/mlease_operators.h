@@ -38,8 +38,8 @@ enum { MLX_I32 = 0, MLX_I64 = 1 };
 int mlx_embedding_lookup(int32_t device, void *stream, int32_t type, const void *table, int64_t n_rows, int64_t width, int64_t ld_table,
                          int32_t id_type, const void *ids, int64_t n_ids, float scale, void *out, int64_t ld_out);
 
-/* grad[v][j] = scale * sum over the t with ids[t] == v of grad_out[t][j], summed in 32 bits in ascending t by parts that depend on the
- * sizes only. accumulate == 0: grad [n_rows][width] is written whole (rows without an id are zero); accumulate != 0: the sums are
+/* grad[v][j] = scale * sum over the t with ids[t] == v of grad_out[t][j], summed in 32 bits in an order that the
+ * sizes and ids decide. accumulate == 0: grad [n_rows][width] is written whole (rows without an id are zero); accumulate != 0: the sums are
  * added to what grad holds (32-bit sum, rounded once) and rows without an id are not touched. grad_type is `type` or MLX_F32. */
 int mlx_embedding_gradient_workspace(int64_t n_rows, int64_t width, int64_t n_ids, size_t *bytes);
 int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const void *grad_out, int64_t ld_grad_out, int32_t id_type, const void *ids,

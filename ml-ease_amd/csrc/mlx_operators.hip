@@ -597,6 +597,135 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
     }
 }
 
+// Few entries: one launch without a sort or a workspace. A workgroup takes an entry and a tile of columns; it goes on if no entry before has the same id,
+// and adds up the rows of all that have it, every group of lanes each groups-th of them, then the groups' sums by halves. Other workgroups write the
+// zeros of the rows that no entry names, told by a bit a row in LDS. Bound by latency (ids, then rows) and by the workgroups that only read the
+// ids, 1.2 ns each: 300 rows of 512 f16 into 8192 rows 6.4 us, by the sort's three launches 12.2 and more around the call. Up to FEW_BLOCKS workgroups
+// (512 rows of 4096 floats: 24 us, 21 by the sort; 128 of them: 14, 18) and FEW entries: of 512 rows of 2048 bf16 into 8192, other ids each, 12 us (16 by
+// the sort), all of one id 21 (17), of 1024 rows 19 (18) and 36 (21). An id of very many rows is the slow case, so tiles are narrower and groups more
+// while that makes FEW_NARROW workgroups at most: 512 rows of 512 bf16 of one id 11 us instead of 17 (other ids 7.5 instead of 6.6).
+constexpr int FEW = 512, FEW_CHUNKS = FEW / 64, FEW_AHEAD = 16, ZERO_ROWS = 4096;
+constexpr int64_t FEW_NARROW = 1024, FEW_BLOCKS = 4096;
+struct FewArgs { int64_t n_rows, width, ldg, ld; uint32_t tiles, sums; float scale; int n, add, lpr, zero_lpr, zero_rows; int64_t zero_cuts, zero_items; };
+
+template <class T, class G, bool NT, bool NARROW>
+__device__ __forceinline__ void few_sum(const T *__restrict__ gout, G *__restrict__ grad, Ids ids, const FewArgs &a, uint64_t *same, uint16_t *list, float (*sums)[Chunk<T>::N])
+{
+    constexpr int E = Chunk<T>::N, AHEAD = FEW_AHEAD;
+    const int t = (int)(blockIdx.x / a.tiles);
+    const int64_t id = id_at(ids, t, a.n_rows);
+    bool on[FEW / 256];
+#pragma unroll
+    for (int r = 0; r < FEW / 256; r++) {
+        const int i = r * 256 + threadIdx.x;
+        on[r] = i < a.n && id_at(ids, i < a.n ? i : 0, a.n_rows) == id;
+        const uint64_t m = __ballot(on[r]);
+        if ((threadIdx.x & 63) == 0) same[i >> 6] = m;
+    }
+    if (id < 0) return;
+    __syncthreads();
+    int before[FEW / 256] = {}, count = 0;
+    bool earlier = false;
+#pragma unroll
+    for (int c = 0; c < FEW_CHUNKS; c++) {
+        const uint64_t m = same[c];
+        const int k = __popcll(m);
+        if (c < t >> 6) earlier |= m != 0;
+        if (c == t >> 6) earlier |= (m & ((1ull << (t & 63)) - 1)) != 0;
+#pragma unroll
+        for (int r = 0; r < FEW / 256; r++)
+            if (c < (r * 256 + (int)threadIdx.x) >> 6) before[r] += k;
+        count += k;
+    }
+    if (earlier) return;
+#pragma unroll
+    for (int r = 0; r < FEW / 256; r++) {
+        const int i = r * 256 + threadIdx.x;
+        if (on[r]) list[before[r] + __popcll(same[i >> 6] & ((1ull << (i & 63)) - 1))] = (uint16_t)i;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & ((1 << a.lpr) - 1), group = threadIdx.x >> a.lpr, groups = 256 >> a.lpr;
+    const int64_t slots = NARROW ? 1 : (a.width + E - 1) / E, slot = ((int64_t)(blockIdx.x % a.tiles) << a.lpr) + lane;
+    const bool mine = slot < slots;
+    const Slot<T> at(mine ? slot : 0, a.width);
+    float sum[E] = {};
+    for (int i0 = group; i0 < count; i0 += AHEAD * groups) {
+        u32x4 raw[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int e = i0 + i * groups;
+            if (e >= count) continue;
+            const T *row = gout + (int64_t)list[e] * a.ldg + at.j;
+            if constexpr (NARROW) {
+                union { u32x4 v; T x[E]; } u;
+                u.v = u32x4(0);
+#pragma unroll
+                for (int k = 0; k < E; k++)
+                    if (k < at.count) u.x[k] = row[k];
+                raw[i] = u.v;
+            } else raw[i] = load_raw<false>(row);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            if (i0 + i * groups >= count) continue;
+            float f[E];
+            unpack<T>(raw[i], f);
+#pragma unroll
+            for (int k = 0; k < E; k++) sum[k] += f[k];
+        }
+    }
+    if (count > 1) {
+#pragma unroll
+        for (int k = 0; k < E; k++) sums[threadIdx.x][k] = sum[k];
+        __syncthreads();
+        for (int half = groups >> 1; half; half >>= 1) {
+            if (group < half)
+#pragma unroll
+                for (int k = 0; k < E; k++) sums[threadIdx.x][k] += sums[threadIdx.x + (half << a.lpr)][k];
+            __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < E; k++) sum[k] = sums[threadIdx.x][k];
+    }
+    if (group == 0 && mine) put_slot<T, G, NT, NARROW>(grad + id * a.ld, at, sum, a.scale, a.add);
+}
+template <class G, bool NT>
+__device__ __forceinline__ void few_zeros(G *__restrict__ grad, Ids ids, const FewArgs &a, uint32_t *named)
+{
+    constexpr int E = Chunk<G>::N, CUT = 4096;
+    const float zero[E] = {};
+    const int lane = threadIdx.x & ((1 << a.zero_lpr) - 1), local = threadIdx.x >> a.zero_lpr, step = 256 >> a.zero_lpr;
+    for (int64_t b = blockIdx.x - a.sums; b < a.zero_items; b += gridDim.x - a.sums) {
+        const int64_t r0 = b / a.zero_cuts * a.zero_rows;
+        const int rows = r0 + a.zero_rows < a.n_rows ? a.zero_rows : (int)(a.n_rows - r0);
+        for (int i = threadIdx.x; i < (rows + 31) / 32; i += 256) named[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.n; i += 256) {
+            const int64_t r = id_at(ids, i, a.n_rows) - r0;
+            if (r >= 0 && r < rows) atomicOr(&named[r >> 5], 1u << (r & 31));
+        }
+        __syncthreads();
+        const int64_t slots = (a.width + E - 1) / E, s0 = b % a.zero_cuts * CUT, s1 = s0 + CUT < slots ? s0 + CUT : slots;
+        for (int r = local; r < rows; r += step) {
+            if (named[r >> 5] >> (r & 31) & 1) continue;
+            G *row = grad + (r0 + r) * a.ld;
+            if (a.width < E) for (int j = 0; j < (int)a.width; j++) row[j] = from_float<G>(0.0f);
+            else for (int64_t s = s0 + lane; s < s1; s += 1 << a.zero_lpr) store_chunk<NT>(row + Slot<G>(s, a.width).j, zero);
+        }
+        __syncthreads();
+    }
+}
+template <class T, class G, bool NT, bool NARROW>
+__global__ __launch_bounds__(256) void k_few_entries(const T *__restrict__ gout, G *__restrict__ grad, Ids ids, FewArgs a)
+{
+    __shared__ uint64_t same[FEW_CHUNKS];
+    __shared__ uint16_t list[FEW];
+    __shared__ float sums[256][Chunk<T>::N];
+    __shared__ uint32_t named[ZERO_ROWS / 32];
+    if (blockIdx.x < a.sums) few_sum<T, G, NT, NARROW>(gout, grad, ids, a, same, list, sums);
+    else few_zeros<G, NT>(grad, ids, a, named);
+}
+
 // ---------------------------------------------------------------------------------------------- log-likelihood of a token
 // The forward pass reads through the caches as usual, so that the backward pass finds in the memory-side cache what that holds of the logits;
 // that pass reads and writes past them (8192 x 32000 bf16, both passes: 174 us so, 212 us with the forward reads non-temporal too, 204 us with
@@ -1137,7 +1266,7 @@ bool streams(int64_t rows, int64_t width, int64_t bytes) { return rows * width >
 // 32000 rows 221 us (frequent ids) and 211 (uniform) instead of 240 and 256, 16384 entries in 32000 rows 109 and 103 instead of 111 and 113; with a
 // quarter of the rows' number in entries 144 and 143 instead of 142 and 153, with an eighth 126 and 127 instead of 121 and 128.
 constexpr int64_t OWNER_WIDTH = 2048;
-struct GradientPlan { SortPlan sort; int lpr; bool owner; int64_t slots, tiles, pieces; size_t key, counts, owners, part, bytes; };
+struct GradientPlan { SortPlan sort; int lpr; bool owner, few; int64_t slots, tiles, pieces; size_t key, counts, owners, part, bytes; };
 GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
 {
     GradientPlan g;
@@ -1151,13 +1280,14 @@ GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
     while (g.lpr < 6 && (1 << g.lpr) < g.slots) g.lpr++;
     g.tiles = ceil_div(g.slots, 1 << g.lpr);
     g.pieces = ceil_div(n, (int64_t)(256 >> g.lpr) * SEG);
+    g.few = n > 0 && n <= FEW && n * g.tiles <= FEW_BLOCKS;
     auto round = [](size_t b) { return (b + 255) / 256 * 256; };
     g.key = round((size_t)n * 4);
     g.counts = n <= ONE_TILE ? 0 : round((size_t)g.sort.tiles * DIGITS * 4);
     g.owner = n > ONE_TILE && width >= OWNER_WIDTH && n >= n_rows / 2;
     g.owners = g.owner ? round((size_t)n_rows * 4) : 0;
     g.part = g.pieces > 1 ? round((size_t)g.pieces * 2 * (size_t)g.slots * (size_t)E * 4) : 0;
-    g.bytes = 4 * g.key + g.counts + g.owners + g.part;
+    g.bytes = g.few ? 0 : 4 * g.key + g.counts + g.owners + g.part;
     return g;
 }
 
@@ -1286,6 +1416,23 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
         constexpr bool NT = decltype(nt)::value, NARROW = decltype(narrow)::value;
         const Ids id = { ids, id_type == MLX_I64 };
         G *out = (G *)grad;
+        if (plan.few) {
+            int lpr = plan.lpr;
+            int64_t tiles = plan.tiles;
+            while (lpr > 0 && n_ids > (256 >> lpr) * FEW_AHEAD && 2 * n_ids * tiles <= FEW_NARROW) tiles = ceil_div(plan.slots, 1 << --lpr);
+            FewArgs f = { n_rows, width, ld_grad_out, ld_grad, (uint32_t)tiles, (uint32_t)(n_ids * tiles), scale, (int)n_ids, accumulate != 0, lpr, 0, 0, 0, 0 };
+            unsigned zeros = 0;
+            if (!accumulate) {
+                const int64_t slots = slots_of(width, Chunk<G>::N);
+                while (f.zero_lpr < 8 && (1 << f.zero_lpr) < slots) f.zero_lpr++;
+                f.zero_rows = (256 >> f.zero_lpr) * (int)std::max<int64_t>(1, 16 / ceil_div(slots, 1 << f.zero_lpr));
+                f.zero_cuts = ceil_div(slots, 4096);
+                f.zero_items = ceil_div(n_rows, f.zero_rows) * f.zero_cuts;
+                zeros = (unsigned)std::min<int64_t>(4096, f.zero_items);
+            }
+            hipLaunchKernelGGL((k_few_entries<T, G, NT, NARROW>), dim3(f.sums + zeros), dim3(256), 0, st, (const T *)grad_out, out, id, f);
+            return 0;
+        }
         // The zeros of grad go along with the sort's launches, each a share of the rows: the few workgroups of the sort run beside them.
         const int shares = n_ids <= ONE_TILE ? 1 : 2 * plan.sort.passes;
         int64_t row = 0;

@@ -69,13 +69,20 @@ def test_lookup_refuses(change):
 def test_gradient_refuses(change):
     L = operators.load_operators()
     need = ctypes.c_size_t()
-    assert L.mlx_embedding_gradient_workspace(8, 16, 5, ctypes.byref(need)) == 0 and need.value > 0
-    a = dict(type=1, grad_out=P, ld_grad_out=16, id_type=1, ids=4 * P, n_ids=5, scale=1.0, accumulate=0, grad_type=1, grad=2 * P, n_rows=8, width=16, ld_grad=16,
+    assert L.mlx_embedding_gradient_workspace(8, 16, 600, ctypes.byref(need)) == 0 and need.value > 0
+    a = dict(type=1, grad_out=P, ld_grad_out=16, id_type=1, ids=4 * P, n_ids=600, scale=1.0, accumulate=0, grad_type=1, grad=2 * P, n_rows=8, width=16, ld_grad=16,
              workspace=8 * P, workspace_bytes=need.value)
     a.update(change)
     assert L.mlx_embedding_gradient(0, None, *[a[k] for k in ("type", "grad_out", "ld_grad_out", "id_type", "ids", "n_ids", "scale", "accumulate", "grad_type", "grad", "n_rows",
                                                               "width", "ld_grad", "workspace", "workspace_bytes")]) == -1
     assert b"mlx_embedding_gradient" in L.mlx_last_error(None)
+
+
+@pytest.mark.parametrize("n,width,needs", [(1, 1, False), (512, 64, False), (513, 64, True), (512, 2048, False), (512, 2049, True), (16, 65536, False), (16, 65537, True)])
+def test_gradient_of_few_entries_needs_no_workspace(n, width, needs):
+    """One launch up to 512 entries and 4096 workgroups of 64 lanes' columns of float32, told by the query for both widths of elements."""
+    need = ctypes.c_size_t()
+    assert operators.load_operators().mlx_embedding_gradient_workspace(100, width, n, ctypes.byref(need)) == 0 and (need.value > 0) == needs
 
 
 @pytest.mark.parametrize("change", [dict(type=9), dict(id_type=3), dict(n_tokens=-1), dict(n_tokens=2 ** 31), dict(n_classes=0), dict(logits=None), dict(logits=P + 1), dict(ld=-1),
@@ -299,6 +306,26 @@ def test_gradient_of_one_id_and_of_none(ops, dtype, n, width):
     k = torch.arange(n, device="cuda")
     for ids in (torch.full((n,), 3, device="cuda"), torch.full((n,), -1, device="cuda"), 2 + 3 * (k % 2), (n - 1 - k), torch.where(k < n // 2, 0, 6)):
         check_gradient(ops.embedding_gradient(go, ids, 7, scale=2.0), go, ids, 7, 2.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,width", [(2, 9000, 1), (63, 4097, 7), (64, 1000, 9), (65, 129, 64), (127, 300, 200), (129, 65, 520), (255, 40, 12), (256, 8192, 3), (257, 31, 8),
+                                          (400, 700, 130), (511, 33, 512), (512, 12289, 2), (512, 500, 24), (512, 20, 2048), (7, 3, 40001), (300, 2049, 33)])
+def test_gradient_of_few_entries(ops, dtype, n, rows, width):
+    """Without the sort: ids all over the rows, of a few rows, of one, of the first and last row, ascending; strided, accumulated, with and without absent ones."""
+    g = rng(n * 7 + width)
+    whole = torch.randn(n, width + 3, generator=g, device="cuda").to(dtype)
+    go, k = whole[:, 1:width + 1], torch.arange(n, device="cuda")
+    for ids in (some_ids(g, n, rows, torch.int64), torch.randint(0, min(rows, 3), (n,), generator=g, device="cuda"), torch.full((n,), rows - 1, device="cuda"),
+                (rows - 1) * (k % 2), k % rows, torch.where(k < n - 1, -1, rows // 2).int()):
+        into = torch.full((rows, width + 5), 9.0, device="cuda", dtype=dtype)
+        check_gradient(ops.embedding_gradient(go, ids, rows, scale=0.75, out=into[:, 2:width + 2]), go, ids, rows, 0.75)
+        assert (into[:, :2] == 9).all() and (into[:, width + 2:] == 9).all()
+        start = torch.randn(rows, width, generator=g, device="cuda")
+        out = start.clone()
+        ops.embedding_gradient(go, ids, rows, out=out, accumulate=True)
+        check_gradient(out, go, ids, rows, 1.0, before=start)
 
 
 @gpu
