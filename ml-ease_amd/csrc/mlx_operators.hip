@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void k_embedding_lookup(const T *__restrict__ 
 }
 
 // ---------------------------------------------------------------------------------------------- gradient of the lookup
-// The entries are sorted by id (stable, so that equal ids keep ascending t), then sums run over the sorted list.
+// More than FEW entries are sorted by id (stable, so that equal ids keep ascending t), then sums run over the sorted list; fewer: k_few_entries.
 //
 // Sort: least significant digit first, 9 bits a pass (two passes up to 262143 rows), absent entries (key n_rows) last. A pass is two launches:
 // counts of the digits in every tile of the list, then every workgroup adds up the other tiles' counts by itself (hence SORT_TILES at most) and
@@ -600,7 +600,7 @@ __global__ __launch_bounds__(256) void k_piece_join(G *__restrict__ grad, SumArg
 // Few entries: one launch without a sort or a workspace. A workgroup takes an entry and a tile of columns; it goes on if no entry before has the same id,
 // and adds up the rows of all that have it, every group of lanes each groups-th of them, then the groups' sums by halves. Other workgroups write the
 // zeros of the rows that no entry names, told by a bit a row in LDS. Bound by latency (ids, then rows) and by the workgroups that only read the
-// ids, 1.2 ns each: 300 rows of 512 f16 into 8192 rows 6.4 us, by the sort's three launches 12.2 and more around the call. Up to FEW_BLOCKS workgroups
+// ids, 1.2 ns each: 300 rows of 512 bf16 into 8192 rows 6.6 us, by the sort's three launches 12.2 and more around the call. Up to FEW_BLOCKS workgroups
 // (512 rows of 4096 floats: 24 us, 21 by the sort; 128 of them: 14, 18) and FEW entries: of 512 rows of 2048 bf16 into 8192, other ids each, 12 us (16 by
 // the sort), all of one id 21 (17), of 1024 rows 19 (18) and 36 (21). An id of very many rows is the slow case, so tiles are narrower and groups more
 // while that makes FEW_NARROW workgroups at most: 512 rows of 512 bf16 of one id 11 us instead of 17 (other ids 7.5 instead of 6.6).
