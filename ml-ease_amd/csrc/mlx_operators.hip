@@ -1232,11 +1232,23 @@ struct OnDevice {                            // the calling thread's device for 
     }
     ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
 };
-int launched(const char *what)
-{
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? MLX_OK : mlxi_fail(MLX_ERR_HIP, "%s: launch failed: %s", what, hipGetErrorString(e));
-}
+// A call's launches, one behind the other. Each one's own status counts (the thread's last error may be an older one of somebody else's), and behind one
+// that failed nothing more is enqueued: the kernels of a call read what those before them write.
+template <class T> struct Same { typedef T type; };
+struct Launches {
+    const char *who;
+    hipStream_t stream;
+    int rc = MLX_OK;
+    template <class... P> void operator()(void (*kernel)(P...), int64_t blocks, int lanes, size_t lds, typename Same<P>::type... args)
+    {
+        if (rc) return;
+        void *at[] = { (void *)&args... };
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3((unsigned)blocks), dim3((unsigned)lanes), at, lds, stream);
+        if (e == hipSuccess) return;
+        (void)hipGetLastError();             // reported here; the thread's next HIP call must not report it again
+        rc = mlxi_fail(MLX_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
+    }
+};
 #define MLX_REFUSE(cond, ...) do { if (cond) return mlxi_fail(MLX_ERR_INVALID, __VA_ARGS__); } while (0)
 
 template <class F> int by_type(int32_t type, F &&f)
@@ -1356,6 +1368,7 @@ int mlx_embedding_lookup(int32_t device, void *stream, int32_t type, const void 
                overlaps(out, span(n_ids, width, ld_out, es), ids, n_ids * is), "%s: out overlaps an input", who);
     OnDevice on(device);
     if (on.rc) return on.rc;
+    Launches launch{ who, (hipStream_t)stream };
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
         return by_flag(streams(n_ids, width, es), [&](auto nt) {
@@ -1364,13 +1377,13 @@ int mlx_embedding_lookup(int32_t device, void *stream, int32_t type, const void 
                 int lpr = 0;
                 while (lpr < 8 && (1 << lpr) < slots) lpr++;
                 const int64_t groups = ceil_div(n_ids, 256 >> lpr);
-                hipLaunchKernelGGL((k_embedding_lookup<T, nt.value, narrow.value>), dim3(grid_of(groups)), dim3(256), 0, (hipStream_t)stream, (const T *)table, n_rows, width,
-                                   ld_table, Ids{ ids, id_type == MLX_I64 }, n_ids, scale, (T *)out, ld_out, lpr, groups);
+                launch(k_embedding_lookup<T, decltype(nt)::value, decltype(narrow)::value>, grid_of(groups), 256, 0, (const T *)table, n_rows, width, ld_table,
+                       Ids{ ids, id_type == MLX_I64 }, n_ids, scale, (T *)out, ld_out, lpr, groups);
                 return 0;
             });
         });
     });
-    return launched(who);
+    return launch.rc;
 }
 
 int mlx_embedding_gradient_workspace(int64_t n_rows, int64_t width, int64_t n_ids, size_t *bytes)
@@ -1404,7 +1417,7 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
     if (n_rows == 0) return MLX_OK;
     OnDevice on(device);
     if (on.rc) return on.rc;
-    hipStream_t st = (hipStream_t)stream;
+    Launches launch{ who, (hipStream_t)stream };
     char *w = (char *)workspace;
     uint32_t *key[2] = { (uint32_t *)w, (uint32_t *)(w + plan.key) }, *pos[2] = { (uint32_t *)(w + 2 * plan.key), (uint32_t *)(w + 3 * plan.key) };
     uint32_t *counts = (uint32_t *)(w + 4 * plan.key);
@@ -1430,7 +1443,7 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
                 f.zero_items = ceil_div(n_rows, f.zero_rows) * f.zero_cuts;
                 zeros = (unsigned)std::min<int64_t>(4096, f.zero_items);
             }
-            hipLaunchKernelGGL((k_few_entries<T, G, NT, NARROW>), dim3(f.sums + zeros), dim3(256), 0, st, (const T *)grad_out, out, id, f);
+            launch(k_few_entries<T, G, NT, NARROW>, f.sums + zeros, 256, 0, (const T *)grad_out, out, id, f);
             return 0;
         }
         // The zeros of grad go along with the sort's launches, each a share of the rows: the few workgroups of the sort run beside them.
@@ -1450,19 +1463,18 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
         int cur = 0;
         if (n_ids <= ONE_TILE) {
             const Zeros<G> z = zeros();
-            hipLaunchKernelGGL((k_sort_one_tile<G, NT>), dim3(1 + blocks), dim3(SORT_THREADS), 0, st, id, (int)n_ids, n_rows, plan.sort.passes, key[0], pos[0], z);
+            launch(k_sort_one_tile<G, NT>, 1 + blocks, SORT_THREADS, 0, id, (int)n_ids, n_rows, plan.sort.passes, key[0], pos[0], z);
         } else
             for (int pass = 0; pass < plan.sort.passes; pass++)
                 by_flag(pass == 0, [&](auto first) {
                     constexpr bool FIRST = decltype(first)::value;
                     const int shift = pass * DIGIT_BITS;
                     Zeros<G> z = zeros();
-                    hipLaunchKernelGGL((k_sort_count<G, NT, FIRST>), dim3(plan.sort.tiles + blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, shift, counts,
-                                       key[cur], owner, z);
+                    launch(k_sort_count<G, NT, FIRST>, plan.sort.tiles + blocks, SORT_THREADS, 0, id, n_ids, n_rows, plan.sort, shift, counts, key[cur], owner, z);
                     z = zeros();
                     const int to = FIRST ? 0 : cur ^ 1;
-                    hipLaunchKernelGGL((k_sort_move<G, NT, FIRST>), dim3(plan.sort.tiles + blocks), dim3(SORT_THREADS), 0, st, id, n_ids, n_rows, plan.sort, shift, counts,
-                                       key[cur], pos[cur], key[to], pos[to], z);
+                    launch(k_sort_move<G, NT, FIRST>, plan.sort.tiles + blocks, SORT_THREADS, 0, id, n_ids, n_rows, plan.sort, shift, counts, key[cur], pos[cur], key[to],
+                           pos[to], z);
                     cur = to;
                     return 0;
                 });
@@ -1470,11 +1482,11 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
         const SumArgs a = { key[cur], pos[cur], n_ids, n_rows, width, ld_grad_out, ld_grad, plan.slots, plan.tiles, plan.pieces, scale, accumulate != 0, plan.lpr, part };
         by_flag(plan.lpr == 6, [&](auto wave) {
             constexpr bool WAVE = decltype(wave)::value && !NARROW;
-            hipLaunchKernelGGL((k_piece_sums<T, G, NT, NARROW, WAVE>), dim3(grid_of(plan.pieces * plan.tiles)), dim3(256),
-                               WAVE ? 0 : (2 * (256 >> plan.lpr) * SEG + 2) * sizeof(uint32_t), st, (const T *)grad_out, out, a);
+            launch(k_piece_sums<T, G, NT, NARROW, WAVE>, grid_of(plan.pieces * plan.tiles), 256, WAVE ? 0 : (2 * (256 >> plan.lpr) * SEG + 2) * sizeof(uint32_t),
+                   (const T *)grad_out, out, a);
             return 0;
         });
-        if (plan.pieces > 1) hipLaunchKernelGGL((k_piece_join<T, G, NT, NARROW>), dim3(grid_of((plan.pieces - 1) * plan.tiles)), dim3(256), 0, st, out, a);
+        if (plan.pieces > 1) launch(k_piece_join<T, G, NT, NARROW>, grid_of((plan.pieces - 1) * plan.tiles), 256, 0, out, a);
         return 0;
     };
     by_type(type, [&](auto t) {
@@ -1482,7 +1494,7 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
             return by_flag(width < Chunk<decltype(t)>::N, [&](auto narrow) { return grad_type == MLX_F32 ? with(t, float(), nt, narrow) : with(t, t, nt, narrow); });
         });
     });
-    return launched(who);
+    return launch.rc;
 }
 
 int mlx_token_loglik_workspace(int64_t n_tokens, int64_t n_classes, size_t *bytes)
@@ -1514,29 +1526,27 @@ int mlx_token_loglik(int32_t device, void *stream, int32_t type, const void *log
                overlaps(stats, 8 * n_tokens, target, is * n_tokens) || overlaps(logp, 4 * n_tokens, stats, 8 * n_tokens), "%s: an output overlaps an input or the other output", who);
     OnDevice on(device);
     if (on.rc) return on.rc;
+    Launches launch{ who, (hipStream_t)stream };
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
-        hipStream_t st = (hipStream_t)stream;
         const T *x = (const T *)logits;
         const Ids y = { target, id_type == MLX_I64 };
         if (plan.parts > 1) {
-            hipLaunchKernelGGL((k_token_loglik_parts<T>), dim3((unsigned)(n_tokens * plan.parts)), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
-                               (RowSum *)workspace);
-            hipLaunchKernelGGL((k_token_loglik_join<T>), dim3((unsigned)n_tokens), dim3(64), 0, st, x, n_tokens, n_classes, ld_logits, y, plan.parts,
-                               (const RowSum *)workspace, logp, stats);
+            launch(k_token_loglik_parts<T>, n_tokens * plan.parts, 256, 0, x, n_tokens, n_classes, ld_logits, y, plan.parts, (RowSum *)workspace);
+            launch(k_token_loglik_join<T>, n_tokens, 64, 0, x, n_tokens, n_classes, ld_logits, y, plan.parts, (const RowSum *)workspace, logp, stats);
             return 0;
         }
         if (plan.lanes == 1024) {
-            hipLaunchKernelGGL((k_token_loglik<T, 1024>), dim3((unsigned)n_tokens), dim3(1024), 0, st, x, n_tokens, n_classes, ld_logits, y, logp, stats);
+            launch(k_token_loglik<T, 1024>, n_tokens, 1024, 0, x, n_tokens, n_classes, ld_logits, y, logp, stats);
             return 0;
         }
         return by_lanes(plan.lanes, [&](auto l) {
             constexpr int LANES = decltype(l)::value;
-            hipLaunchKernelGGL((k_token_loglik<T, LANES>), dim3(grid_of(ceil_div(n_tokens, 256 / LANES))), dim3(256), 0, st, x, n_tokens, n_classes, ld_logits, y, logp, stats);
+            launch(k_token_loglik<T, LANES>, grid_of(ceil_div(n_tokens, 256 / LANES)), 256, 0, x, n_tokens, n_classes, ld_logits, y, logp, stats);
             return 0;
         });
     });
-    return launched(who);
+    return launch.rc;
 }
 
 int mlx_token_loglik_gradient(int32_t device, void *stream, int32_t type, const void *logits, int64_t n_tokens, int64_t n_classes, int64_t ld_logits,
@@ -1559,20 +1569,20 @@ int mlx_token_loglik_gradient(int32_t device, void *stream, int32_t type, const 
                "%s: dlogits overlaps an input", who);
     OnDevice on(device);
     if (on.rc) return on.rc;
+    Launches launch{ who, (hipStream_t)stream };
     by_type(type, [&](auto t) {
         typedef decltype(t) T;
         const LoglikPlan plan = loglik_plan(es, n_tokens, n_classes);
         return by_flag(plan.grad_lanes == 256 && streams(n_tokens, n_classes, 2 * es), [&](auto nt) {
             return by_lanes(plan.grad_lanes, [&](auto l) {
                 constexpr int LANES = decltype(l)::value;
-                hipLaunchKernelGGL((k_token_loglik_gradient<T, nt.value, LANES>), dim3(grid_of(ceil_div(n_tokens * plan.grad_parts, 256 / LANES))), dim3(256), 0, (hipStream_t)stream,
-                                   (const T *)logits, n_tokens, n_classes, ld_logits, Ids{ target, id_type == MLX_I64 }, stats, grad_logp, (T *)dlogits, ld_dlogits,
-                                   (int64_t)plan.grad_parts);
+                launch(k_token_loglik_gradient<T, decltype(nt)::value, LANES>, grid_of(ceil_div(n_tokens * plan.grad_parts, 256 / LANES)), 256, 0, (const T *)logits, n_tokens,
+                       n_classes, ld_logits, Ids{ target, id_type == MLX_I64 }, stats, grad_logp, (T *)dlogits, ld_dlogits, (int64_t)plan.grad_parts);
                 return 0;
             });
         });
     });
-    return launched(who);
+    return launch.rc;
 }
 
 int mlx_preference_loss_workspace(int64_t n_tokens, int64_t n_pairs, size_t *bytes)
@@ -1611,17 +1621,17 @@ int mlx_preference_loss(int32_t device, void *stream, const float *logp, const f
     }
     OnDevice on(device);
     if (on.rc) return on.rc;
+    Launches launch{ who, (hipStream_t)stream };
     const PrefArgs a = { logp, ref_logp, n_tokens, seq_ptr, n_pairs, beta, smoothing, scale, mean != 0, mask, weight, offset, loss, pair_loss, margin, ratio, grad,
                          (double *)((char *)workspace + plan.sums), (double *)workspace, plan.parts };
-    hipStream_t st = (hipStream_t)stream;
     if (plan.parts > 1) {
-        hipLaunchKernelGGL(k_preference_part_sums, dim3((unsigned)(2 * n_pairs * plan.parts)), dim3(256), 0, st, a);
-        hipLaunchKernelGGL(k_preference_part_gradients, dim3((unsigned)(2 * n_pairs * plan.parts)), dim3(256), 0, st, a);
-    } else if (plan.lanes == 1) hipLaunchKernelGGL(k_preference_short<1>, dim3((unsigned)plan.groups), dim3(256), 0, st, a);
-    else if (plan.lanes == 8) hipLaunchKernelGGL(k_preference_short<8>, dim3((unsigned)plan.groups), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_preference_pairs, dim3((unsigned)plan.groups), dim3(512), 0, st, a);
-    if (plan.groups > 1 || plan.parts > 1) hipLaunchKernelGGL(k_preference_total, dim3(1), dim3(256), 0, st, a, plan.groups);
-    return launched(who);
+        launch(k_preference_part_sums, 2 * n_pairs * plan.parts, 256, 0, a);
+        launch(k_preference_part_gradients, 2 * n_pairs * plan.parts, 256, 0, a);
+    } else if (plan.lanes == 1) launch(k_preference_short<1>, plan.groups, 256, 0, a);
+    else if (plan.lanes == 8) launch(k_preference_short<8>, plan.groups, 256, 0, a);
+    else launch(k_preference_pairs, plan.groups, 512, 0, a);
+    if (plan.groups > 1 || plan.parts > 1) launch(k_preference_total, 1, 256, 0, a, plan.groups);
+    return launch.rc;
 }
 
 }  // extern "C"

@@ -1,9 +1,12 @@
 """The operators on token ids, logits and pairs of answers (ml-ease_amd/operators.py, include/mlease_operators.h) against plain
 64-bit computations. Tolerances count roundings: u = 2^-24 for a 32-bit operation, half a step of the result's type for the last one."""
 import ctypes
+import json
 import math
 import os
 import re
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -188,6 +191,81 @@ def test_no_device():
     ops = _on_cpu()
     with pytest.raises(RuntimeError, match="mlease_hip error -3"):
         ops.embedding_lookup(torch.zeros(4, 6), torch.zeros(5, dtype=torch.int64))
+
+
+# The HIP runtime's part of a call, as far as the entry points use it: launches are counted and not made, the FAIL-th fails, and the thread's last error
+# is what an earlier call of somebody else's left there.
+FAKE_RUNTIME = r"""
+#include <stdlib.h>
+static int launches, last = 700;
+int launches_made(void) { return launches; }
+void start_again(void) { launches = 0; last = 700; }
+int hipGetDevice(int *d) { *d = 0; return 0; }
+int hipSetDevice(int d) { (void)d; return 0; }
+int hipGetLastError(void) { int e = last; last = 0; return e; }
+int hipPeekAtLastError(void) { return last; }
+struct d3 { unsigned x, y, z; };
+int __hipPushCallConfiguration(struct d3 g, struct d3 b, size_t n, void *s) { (void)g; (void)b; (void)n; (void)s; return 0; }
+int __hipPopCallConfiguration(struct d3 *g, struct d3 *b, size_t *n, void **s)
+{ struct d3 one = { 1, 1, 1 }; *g = *b = one; *n = 0; *s = 0; return 0; }
+int hipLaunchKernel(const void *f, struct d3 g, struct d3 b, void **a, size_t n, void *s)
+{
+    (void)f; (void)g; (void)b; (void)a; (void)n; (void)s;
+    return ++launches == atoi(getenv("FAIL")) ? last = 719 : 0;
+}
+"""
+CALLS_ON_IT = """
+import ctypes, json, sys
+fake = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
+import mlease_amd
+from mlease_amd import operators
+L = operators.load_operators()
+P, need, out = 1 << 30, ctypes.c_size_t(), {}
+def call(name, f, *a):
+    fake.start_again()
+    out[name] = [f(*a), fake.launches_made(), fake.hipPeekAtLastError(), L.mlx_last_error(None).decode()]
+call("lookup", L.mlx_embedding_lookup, 0, None, 1, P, 8, 16, 16, 1, 2 * P, 5, 1.0, 3 * P, 16)
+L.mlx_embedding_gradient_workspace(300000, 64, 60000, ctypes.byref(need))
+call("gradient", L.mlx_embedding_gradient, 0, None, 1, P, 64, 1, 2 * P, 60000, 1.0, 1, 0, 3 * P, 300000, 64, 64, 8 * P, need.value)
+L.mlx_token_loglik_workspace(3, 2000000, ctypes.byref(need))
+call("loglik", L.mlx_token_loglik, 0, None, 1, P, 3, 2000000, 2000000, 1, 2 * P, 3 * P, 4 * P, 8 * P, need.value)
+call("dlogits", L.mlx_token_loglik_gradient, 0, None, 1, P, 3, 100, 100, 1, 2 * P, 3 * P, 4 * P, P, 100)
+L.mlx_preference_loss_workspace(100000, 2, ctypes.byref(need))
+call("preference", L.mlx_preference_loss, 0, None, P, None, 100000, 2 * P, 2, 0.1, 0.0, 1.0, 0, None, None, None, 3 * P, 4 * P, 5 * P, 6 * P, 7 * P, 8 * P, need.value)
+print(json.dumps(out))
+"""
+
+
+@pytest.fixture(scope="module")
+def on_fake_runtime(tmp_path_factory):
+    d = tmp_path_factory.mktemp("runtime")
+    (d / "fake.c").write_text(FAKE_RUNTIME)
+    subprocess.check_call(["gcc", "-shared", "-fPIC", "-O1", "-w", "-o", str(d / "fake.so"), str(d / "fake.c")])
+
+    def calls(fail):
+        done = subprocess.run([sys.executable, "-c", CALLS_ON_IT, str(d / "fake.so")], cwd=ROOT, env=dict(os.environ, FAIL=str(fail)), capture_output=True, text=True, timeout=300)
+        assert done.returncode == 0, done.stderr
+        return json.loads(done.stdout)
+    return calls
+
+
+def test_an_error_that_was_there_before_is_not_a_calls(on_fake_runtime):
+    """A thread's last error stays until it is read: one that somebody else left is neither reported by a call whose launches all succeeded (its caller
+    would make it again, and accumulate twice) nor taken from its owner."""
+    for name, (rc, launches, last, _) in on_fake_runtime(0).items():
+        assert rc == 0 and last == 700, name
+        assert launches == {"lookup": 1, "gradient": 8, "loglik": 2, "dlogits": 1, "preference": 3}[name]
+
+
+@pytest.mark.parametrize("fail", [1, 2, 3, 5, 7, 8])
+def test_nothing_is_launched_behind_a_launch_that_failed(on_fake_runtime, fail):
+    """The sums take row numbers from what the sort has written: without the sort they must not run."""
+    most = on_fake_runtime(0)
+    for name, (rc, launches, last, text) in on_fake_runtime(fail).items():
+        if fail > most[name][1]:
+            assert rc == 0 and launches == most[name][1]
+        else:
+            assert rc == -2 and launches == fail and last == 0 and "launch failed" in text, name
 
 
 # ---------------------------------------------------------------------------------------------- lookup
