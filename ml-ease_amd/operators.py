@@ -124,7 +124,10 @@ class HipOperators:
         w = self._torch.empty(need.value, dtype=self._torch.uint8, device=self._at)      # torch's blocks are aligned to 512 bytes
         return w, w.data_ptr(), need.value
 
-    def _ck(self, rc):
+    def _ck(self, rc, written=None):
+        """written: the caller's tensor that a call's kernels write; torch is told, so that a graph that kept it for a backward pass notices."""
+        if written is not None and rc in (0, -2):        # (-2: some of the launches may have been made)
+            self._torch.autograd.graph.increment_version(written)
         if rc != 0:
             raise RuntimeError("mlease_hip error %d: %s" % (rc, self.L.mlx_last_error(None).decode()))
 
@@ -135,8 +138,9 @@ class HipOperators:
         ip, it = self._ids(ids, "ids")
         rows, width = table.shape
         n = ids.shape[0]
+        given = out
         out, op, ldo = self._output(out, (n, width), table.dtype)
-        self._ck(self.L.mlx_embedding_lookup(self.device, self._stream(), self._types[table.dtype], tp, rows, width, ld, it, ip, n, scale, op, ldo))
+        self._ck(self.L.mlx_embedding_lookup(self.device, self._stream(), self._types[table.dtype], tp, rows, width, ld, it, ip, n, scale, op, ldo), given)
         return out
 
     def embedding_gradient(self, grad_out, ids, n_rows: int, scale: float = 1.0, out=None, accumulate: bool = False, dtype=None):
@@ -150,10 +154,11 @@ class HipOperators:
         dtype = dtype or (grad_out.dtype if out is None else out.dtype)
         if dtype not in self._types:
             raise ValueError("grad must be of grad_out's type or float32, not %s" % dtype)
+        given = out
         out, op, ldo = self._output(out, (n_rows, width), dtype)
         keep, wp, wb = self._workspace(self.L.mlx_embedding_gradient_workspace, n_rows, width, n)
         self._ck(self.L.mlx_embedding_gradient(self.device, self._stream(), self._types[grad_out.dtype], gp, ldg, it, ip, n, scale, bool(accumulate),
-                                               self._types[dtype], op, n_rows, width, ldo, wp, wb))
+                                               self._types[dtype], op, n_rows, width, ldo, wp, wb), given)
         return out
 
     # -- log-likelihood ---------------------------------------------------------------------------
@@ -177,8 +182,9 @@ class HipOperators:
         if tuple(stats.shape) != (n, 2) or not stats.is_contiguous():
             raise ValueError("stats must be what token_loglik gave for these logits, [%d, 2]" % n)
         sp = self._vector(stats.view(-1), "stats", 2 * n, self._f32)
+        given = out
         out, op, ldo = self._output(out, (n, classes), logits.dtype)
-        self._ck(self.L.mlx_token_loglik_gradient(self.device, self._stream(), self._types[logits.dtype], lp, n, classes, ld, it, ip, sp, gp, op, ldo))
+        self._ck(self.L.mlx_token_loglik_gradient(self.device, self._stream(), self._types[logits.dtype], lp, n, classes, ld, it, ip, sp, gp, op, ldo), given)
         return out
 
     # -- preference -------------------------------------------------------------------------------

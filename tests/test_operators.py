@@ -184,6 +184,54 @@ def test_binding_refuses():
             call()
 
 
+def _on_nothing(rc=0):
+    """The binding with tensors of this host and a library that only says what it was called for: every launch gives rc."""
+    ops = _on_cpu()
+    real, ops.called = ops.L, []
+
+    class Library:
+        def __getattr__(self, name):
+            if name.endswith("_workspace") or name == "mlx_last_error":
+                return getattr(real, name)
+            return lambda *a: ops.called.append(name) or rc
+    ops.L = Library()
+    return ops
+
+
+@pytest.mark.parametrize("rc", [0, -1, -2])
+def test_a_tensor_written_in_place_gets_a_new_version(rc):
+    """torch's version counter of the caller's `out`, also where it is a view or the logits themselves; a call that was refused wrote nothing."""
+    ops = _on_nothing(rc)
+    i, f, stats = torch.zeros(5, dtype=torch.int64), torch.zeros(5), torch.zeros(5, 2)
+    whole, logits = torch.zeros(5, 9), torch.zeros(5, 6)
+    for out, call in ((whole, lambda: ops.embedding_lookup(torch.zeros(4, 6), i, out=whole[:, 1:7])),
+                      (whole, lambda: ops.embedding_gradient(torch.zeros(5, 6), i, 5, out=whole[:, :6])),
+                      (whole, lambda: ops.embedding_gradient(torch.zeros(5, 6), i, 5, out=whole[:, :6], accumulate=True)),
+                      (logits, lambda: ops.token_loglik_gradient(logits, i, stats, f, out=logits)),
+                      (logits, lambda: ops.token_loglik_gradient(logits, i, stats, f, out=logits.detach())),
+                      (whole, lambda: ops.token_loglik_gradient(logits, i, stats, f, out=whole[:, :6]))):
+        before = out._version, stats._version, f._version
+        if rc:
+            with pytest.raises(RuntimeError, match="mlease_hip error %d" % rc):
+                call()
+        else:
+            call()
+        assert (out._version > before[0]) == (rc != -1) and (stats._version, f._version) == before[1:]
+
+
+@gpu
+def test_an_overwritten_tensor_that_a_graph_kept_is_noticed(ops):
+    """A soft cap keeps its result for its backward pass; the gradient written over it must not pass for it."""
+    w = torch.randn(7, 50, device="cuda", requires_grad=True)
+    target = torch.arange(7, device="cuda")
+    logits = torch.tanh(w)
+    plain = logits.detach()
+    logp, stats = ops.token_loglik(plain, target)
+    ops.token_loglik_gradient(plain, target, stats, torch.ones(7, device="cuda"), out=plain)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        logits.sum().backward()
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="asks what happens without a device")
 def test_no_device():
     with pytest.raises(RuntimeError, match="no HIP device"):
