@@ -13,7 +13,9 @@ gradient (``HipAdmmEngine.test_loglik_sums`` for two), and the logistic loss wit
     ...
     ops.embedding_gradient(dx, ids, n_rows, scale=math.sqrt(width), out=table_grad, accumulate=True)
 
-Gradients are calls of their own, as everywhere in this package: nothing records them. Every call enqueues its work on torch's
+Gradients are calls of their own, as everywhere in this package: nothing records them. A tensor that automatic differentiation
+follows is refused, since its gradient would be missing without a word; layers recorded by torch meet these calls at
+`logits.detach()` and take the gradient from there with `logits.backward(dlogits)`. Every call enqueues its work on torch's
 current stream of the device and returns; it allocates its outputs and workspace from torch on that stream, so that it can be
 captured into a graph and made from several threads and streams. Tensors that were written on another stream need the caller's
 event, as for any torch operation. There is no CPU fallback.
@@ -73,10 +75,18 @@ class HipOperators:
         self._id_types = {torch.int32: 0, torch.int64: 1}
         self._f32 = torch.float32
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # the stream's handle without the object around it: 2 us of a call
+        self._forward = torch.autograd.forward_ad
         at, device = self._at, self.device
         self._stream = (lambda: raw(device)) if raw else (lambda: torch.cuda.current_stream(at).cuda_stream)
 
     # -- checks -----------------------------------------------------------------------------------
+    def _unrecorded(self, t, what):
+        """Nothing records these calls: what came back for a tensor that automatic differentiation follows would silently lack its gradient."""
+        if t.requires_grad and self._torch.is_grad_enabled():
+            raise ValueError("%s requires a gradient, which these calls do not record: pass it detached (gradients are calls of their own)" % what)
+        if self._forward._current_level >= 0 and self._forward.unpack_dual(t).tangent is not None:
+            raise ValueError("%s carries a forward-mode tangent, which these calls do not follow" % what)
+
     def _matrix(self, t, what):
         """(pointer, ld) of a 2-D tensor of this device whose rows are contiguous."""
         if t.dim() != 2 or t.dtype not in self._types:
@@ -85,9 +95,11 @@ class HipOperators:
             raise ValueError("%s is on %s, these operators are on %s" % (what, t.device, self._at))
         if t.shape[1] > 1 and t.stride(1) != 1:
             raise ValueError("the rows of %s must be contiguous (strides %s)" % (what, tuple(t.stride())))
+        self._unrecorded(t, what)
         return t.data_ptr(), t.stride(0)
 
     def _vector(self, t, what, n, dtype):
+        self._unrecorded(t, what)
         if t.dtype is dtype and t.shape == (n,) and t.device == self._at and t.is_contiguous():
             return t.data_ptr()
         if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype:

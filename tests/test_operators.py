@@ -184,6 +184,38 @@ def test_binding_refuses():
             call()
 
 
+def _float_arguments(ops):
+    """For each floating tensor that a call takes: its name, the call with that tensor replaced, and a tensor that it takes."""
+    i, seq = torch.zeros(5, dtype=torch.int64), torch.tensor([0, 2, 5])
+    t, f, stats, pair = torch.zeros(4, 6), torch.zeros(5), torch.zeros(5, 2), torch.zeros(1)
+    rows = torch.zeros(5, 6)
+    return [
+        ("table", lambda x: ops.embedding_lookup(x, i), t), ("out", lambda x: ops.embedding_lookup(t, i, out=x), rows),
+        ("grad_out", lambda x: ops.embedding_gradient(x, i, 3), rows), ("out", lambda x: ops.embedding_gradient(rows, i, 4, out=x), t),
+        ("out", lambda x: ops.embedding_gradient(rows, i, 4, out=x, accumulate=True), t), ("logits", lambda x: ops.token_loglik(x, i), rows),
+        ("logits", lambda x: ops.token_loglik_gradient(x, i, stats, f), rows), ("stats", lambda x: ops.token_loglik_gradient(rows, i, x, f), stats),
+        ("grad_logp", lambda x: ops.token_loglik_gradient(rows, i, stats, x), f), ("out", lambda x: ops.token_loglik_gradient(rows, i, stats, f, out=x), rows.clone()),
+        ("logp", lambda x: ops.preference_loss(x, None, seq), f), ("ref_logp", lambda x: ops.preference_loss(f, x, seq), f.clone()),
+        ("weight", lambda x: ops.preference_loss(f, None, seq, weight=x), pair), ("offset", lambda x: ops.preference_loss(f, None, seq, offset=x), pair.clone())]
+
+
+def test_what_automatic_differentiation_follows_is_refused():
+    """A gradient that would be missing without a word; where torch itself records nothing, or from a detached tensor, the call is made."""
+    for what, call, tensor in _float_arguments(_on_nothing()):
+        call(tensor)
+        with pytest.raises(ValueError, match="%s requires a gradient" % what):
+            call(tensor.clone().requires_grad_())
+        with pytest.raises(ValueError, match="%s requires a gradient" % what):
+            call(tensor.clone().requires_grad_() * 2)
+        call(tensor.clone().requires_grad_().detach())
+        with torch.no_grad():
+            call(tensor.clone().requires_grad_())
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(ValueError, match="%s carries a forward-mode tangent" % what):
+                call(torch.autograd.forward_ad.make_dual(tensor.clone(), torch.ones_like(tensor)))
+            call(tensor)
+
+
 def _on_nothing(rc=0):
     """The binding with tensors of this host and a library that only says what it was called for: every launch gives rc."""
     ops = _on_cpu()
