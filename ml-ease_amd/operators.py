@@ -80,12 +80,14 @@ class HipOperators:
         self._stream = (lambda: raw(device)) if raw else (lambda: torch.cuda.current_stream(at).cuda_stream)
 
     # -- checks -----------------------------------------------------------------------------------
-    def _unrecorded(self, t, what):
+    def _as_stored(self, t, what):
         """Nothing records these calls: what came back for a tensor that automatic differentiation follows would silently lack its gradient."""
         if t.requires_grad and self._torch.is_grad_enabled():
             raise ValueError("%s requires a gradient, which these calls do not record: pass it detached (gradients are calls of their own)" % what)
         if self._forward._current_level >= 0 and self._forward.unpack_dual(t).tangent is not None:
             raise ValueError("%s carries a forward-mode tangent, which these calls do not follow" % what)
+        if t.is_neg():
+            raise ValueError("%s is a view that torch negates when it is read: pass its resolve_neg()" % what)
 
     def _matrix(self, t, what):
         """(pointer, ld) of a 2-D tensor of this device whose rows are contiguous."""
@@ -95,11 +97,11 @@ class HipOperators:
             raise ValueError("%s is on %s, these operators are on %s" % (what, t.device, self._at))
         if t.shape[1] > 1 and t.stride(1) != 1:
             raise ValueError("the rows of %s must be contiguous (strides %s)" % (what, tuple(t.stride())))
-        self._unrecorded(t, what)
+        self._as_stored(t, what)
         return t.data_ptr(), t.stride(0)
 
     def _vector(self, t, what, n, dtype):
-        self._unrecorded(t, what)
+        self._as_stored(t, what)
         if t.dtype is dtype and t.shape == (n,) and t.device == self._at and t.is_contiguous():
             return t.data_ptr()
         if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype:

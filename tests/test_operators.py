@@ -216,6 +216,24 @@ def test_what_automatic_differentiation_follows_is_refused():
             call(tensor)
 
 
+def test_views_that_torch_negates_are_refused():
+    """The memory of imag(conj(z)) holds the negatives of its values."""
+    ops = _on_nothing()
+    z = torch.complex(torch.ones(4, 1), torch.ones(4, 1)).conj()
+    lazy, seq = torch.imag(z), torch.zeros(3, dtype=torch.int64)
+    assert lazy.is_neg()
+    for x in (lazy, lazy[:1]):
+        i = torch.zeros(x.shape[0], dtype=torch.int64)
+        with pytest.raises(ValueError, match="negates"):
+            ops.embedding_lookup(x, i)
+        with pytest.raises(ValueError, match="negates"):
+            ops.embedding_lookup(torch.zeros(9, 1), i, out=x)
+        ops.embedding_lookup(x.resolve_neg(), i)
+    with pytest.raises(ValueError, match="negates"):
+        ops.preference_loss(lazy[0], None, seq)
+    ops.preference_loss(lazy[0].resolve_neg(), None, seq)
+
+
 def _on_nothing(rc=0):
     """The binding with tensors of this host and a library that only says what it was called for: every launch gives rc."""
     ops = _on_cpu()
