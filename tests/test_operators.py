@@ -697,6 +697,96 @@ def test_loglik_of_likely_targets(ops, dtype, classes):
     within(d, p_not, p_not * (err * 1.01 + 8 * U) + half_step(p_not, dtype) * (1 + 1e-6) + 2.0 ** -126)
 
 
+ONE_PART = 1.0 - 1.44269502162933 / 1.4426950408889634        # what log2 e as one 32-bit number lacks: 1.33e-8
+MEAN_LOSS = 3.4e-9                                             # of a v_exp_f32, on average
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_loglik_of_targets_far_above(ops, dtype):
+    """Two classes: log p = -log(1 + exp(-d)) with the digits of the one exponential that it is made of. That is off by 2 u (v_exp_f32: one step) and
+    0.18 u (its argument of at most 1/2, rounded), the mean loss that is put back by 0.06 u, the logarithm by nothing, and the result is rounded: u."""
+    g = rng(31)
+    n = 100000
+    x = torch.randn(n, 2, generator=g, device="cuda")
+    target = torch.randint(0, 2, (n,), generator=g, device="cuda")
+    x[torch.arange(n, device="cuda"), target] = torch.rand(n, generator=g, device="cuda") * 72 + 5
+    x = x.to(dtype)
+    v = x.double().gather(1, target[:, None])[:, 0] - x.double().gather(1, 1 - target[:, None])[:, 0]
+    want = -torch.log1p(torch.exp(-v))
+    got, stats = ops.token_loglik(x, target)
+    within(got, want, want.abs() * 3.25 * U)
+    within(stats[:, 1], -want, want.abs() * 3.25 * U)
+
+
+@gpu
+def test_loglik_has_no_bias_of_one_exponential(ops):
+    """The mean of the relative error over 200000 rows of two classes, targets 1 to 12 above: 3.6e-8 rms (v_exp_f32 2.6e-8, rounding 2.5e-8) leave 8e-11;
+    half the mean loss is allowed, so that its correction left out, or of the wrong sign, is seen."""
+    g = rng(32)
+    x = torch.zeros(200000, 2, device="cuda")
+    x[:, 0] = torch.rand(200000, generator=g, device="cuda") * 11 + 1
+    want = -torch.log1p(torch.exp(-x[:, 0].double()))
+    off = ops.token_loglik(x, torch.zeros(200000, dtype=torch.int64, device="cuda"))[0].double() / want - 1
+    assert off.pow(2).mean().sqrt() < 5e-8
+    assert abs(off.mean()) < MEAN_LOSS / 2 < abs(off.mean() - MEAN_LOSS)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,n,classes", [(torch.bfloat16, 8192, 32000), (torch.float32, 8192, 32000), (torch.bfloat16, 4096, 128000), (torch.float16, 4000, 200003)])
+def test_loglik_sums_have_no_bias(ops, dtype, n, classes):
+    """Likely targets of many classes, log p = -log(1 + R): relative errors of R are those of the others' sum. On average over thousands of rows they are off by
+    two exponentials' mean loss at most (a term's own, its lane's rescaling and the joining of lanes, one of them put back: 7e-9), and, 16-bit logits near
+    the maximum being a few dozen values, by the error of v_exp_f32 over those (2.6e-8 / sqrt(50)): 2e-8 are allowed. log2 e in one part is off by 1.33e-8
+    of the mean distance to the maximum, more than twice that. The rms is that of a rounding, of v_exp_f32 and of the lanes' sums: u."""
+    g = rng(classes)
+    off, one_part = [], []
+    for a in range(0, n, 512):
+        x = torch.randn(min(512, n - a), classes, generator=g, device="cuda").mul_(2)
+        x[:, 7] = -1e4
+        x[:, 7] = torch.logsumexp(x, 1) + 6
+        x = x.to(dtype)
+        got = ops.token_loglik(x, torch.full((x.shape[0],), 7, device="cuda"))[0].double()
+        for b in range(0, x.shape[0], 128):
+            v = x[b:b + 128].double()
+            value = v[:, 7:8].clone()
+            v[:, 7] = -math.inf
+            top = v.amax(1, keepdim=True)
+            e = (v - top).exp()
+            mean_t = torch.where(e > 0, e * (top - v), 0.0).sum(1) / e.sum(1)
+            R = e.sum(1) * (top - value)[:, 0].exp()
+            off.append(got[b:b + 128] / -torch.log1p(R) - 1)
+            one_part.append(got[b:b + 128] / -torch.log1p(R * (1 + ONE_PART * mean_t)) - 1)       # (smaller |t| in the exponent: larger terms)
+    off, one_part = torch.cat(off), torch.cat(one_part)
+    assert off.pow(2).mean().sqrt() < U
+    assert abs(off.mean()) < 2e-8 < abs(one_part.mean())
+
+
+@gpu
+def test_margin_of_a_long_answer(ops):
+    """One answer of 39000 tokens against one of 1000, from their logits, under a reference model that is near: the margin adds up the errors of 40000 log p. The
+    roundings add like a random walk (4 of its deviations allowed), and what every row's sum has alike, 2e-8 at most, by the difference of the lengths."""
+    g = rng(33)
+    n, classes, beta = 40000, 4000, 0.125
+    x = torch.randn(n, classes, generator=g, device="cuda").mul_(2).to(torch.bfloat16)
+    target = torch.randint(0, classes, (n,), generator=g, device="cuda")
+    logp, _ = ops.token_loglik(x, target)
+    want, mean_t = torch.empty(n, dtype=torch.float64, device="cuda"), torch.empty(n, dtype=torch.float64, device="cuda")
+    for a in range(0, n, 4000):
+        v, at = x[a:a + 4000].double(), target[a:a + 4000, None]
+        want[a:a + 4000] = (v.gather(1, at) - v.logsumexp(1, keepdim=True))[:, 0]
+        p = v.softmax(1)
+        mean_t[a:a + 4000] = (p * (v.amax(1, keepdim=True) - v)).sum(1)
+    ref = (want + 0.1 * torch.randn(n, generator=g, device="cuda")).float()
+    seq = torch.tensor([0, 39000, 40000], device="cuda")
+    margin = float(ops.preference_loss(logp, ref, seq, beta=beta).margin)
+    sign = torch.where(torch.arange(n, device="cuda") < 39000, 1.0, -1.0).double()
+    exact = beta * float(((want - ref.double()) * sign).sum())
+    allowed = beta * (4 * math.sqrt(n / 3) * float(half_step(want, torch.float32).pow(2).mean().sqrt()) + 38000 * 2e-8) + abs(exact) * U
+    assert abs(margin - exact) <= allowed
+    assert beta * ONE_PART * float((mean_t * sign).sum()) > allowed          # what log2 e in one part would add
+
+
 @gpu
 def test_loglik_of_nothing(ops):
     x = torch.zeros(0, 9, device="cuda")
