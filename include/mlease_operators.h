@@ -67,7 +67,7 @@ int mlx_token_loglik_gradient(int32_t device, void *stream, int32_t type, const 
  *   loss = sum_p scale weight[p] pair_loss[p],   grad[t] = d loss / d logp[t]   (0 for tokens of no sequence)
  * ref_logp NULL = 0; mask (one byte per token, 0 = the token does not count: its logp and ref_logp are not looked at, grad 0) NULL = all
  * count; weight (>= 0; a pair of weight 0 adds nothing) NULL = 1; offset NULL = 0. margin, ratio and grad may be NULL. Sums are in 64 bits.
- * loss is one float, pair_loss and margin n_pairs, ratio 2 n_pairs, grad n_tokens. */
+ * loss is one float, pair_loss and margin n_pairs, ratio 2 n_pairs, grad n_tokens. The workspace is never more than 16384 + 8 n_pairs bytes. */
 int mlx_preference_loss_workspace(int64_t n_tokens, int64_t n_pairs, size_t *bytes);
 int mlx_preference_loss(int32_t device, void *stream, const float *logp, const float *ref_logp, int64_t n_tokens, const int64_t *seq_ptr,
                         int64_t n_pairs, float beta, float smoothing, float scale, int32_t mean, const uint8_t *mask, const float *weight,

@@ -97,12 +97,14 @@ class HipOperators:
             raise ValueError("%s is on %s, these operators are on %s" % (what, t.device, self._at))
         if t.shape[1] > 1 and t.stride(1) != 1:
             raise ValueError("the rows of %s must be contiguous (strides %s)" % (what, tuple(t.stride())))
-        self._as_stored(t, what)
+        if t.requires_grad or self._forward._current_level >= 0 or t.is_neg():
+            self._as_stored(t, what)
         return t.data_ptr(), t.stride(0)
 
     def _vector(self, t, what, n, dtype):
-        self._as_stored(t, what)
-        if t.dtype is dtype and t.shape == (n,) and t.device == self._at and t.is_contiguous():
+        if t.requires_grad or self._forward._current_level >= 0 or t.is_neg():
+            self._as_stored(t, what)
+        if t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.device == self._at and t.is_contiguous():
             return t.data_ptr()
         if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype:
             raise ValueError("%s must be a vector of %d %s, not %s %s" % (what, n, dtype, tuple(t.shape), t.dtype))
@@ -217,15 +219,13 @@ class HipOperators:
         mp = None if mask is None else self._vector(mask, "mask", n, torch.uint8 if mask.dtype == torch.uint8 else torch.bool)
         wp = None if weight is None else self._vector(weight, "weight", pairs, f32)
         fp = None if offset is None else self._vector(offset, "offset", pairs, f32)
-        # the workspace and the few values of every pair in one block, the gradient in one of its own
-        need = C.c_size_t()
-        self._ck(self.L.mlx_preference_loss_workspace(n, pairs, C.byref(need)))
-        kb = need.value
-        few = torch.empty((kb + 3) // 4 + 4 * pairs + 1, dtype=f32, device=self._at)
-        _, ratio, pair_loss, margin, loss = few.split(((kb + 3) // 4, 2 * pairs, pairs, pairs, 1))
-        kp = few.data_ptr()
-        at = kp + (kb + 3) // 4 * 4
-        g = torch.empty(n, dtype=f32, device=self._at) if grad else None
-        self._ck(self.L.mlx_preference_loss(self.device, self._stream(), lp, rp, n, qp, pairs, beta, smoothing, scale, bool(mean), mp, wp, fp, at + 16 * pairs,
-                                            at + 8 * pairs, at + 12 * pairs, at, None if g is None else g.data_ptr(), kp, kb))
-        return PreferenceResult(loss.view(()), pair_loss, margin, ratio, g)
+        # The pairs' values in one block (tensors of their own, not views: each can be written and kept without the others), the loss and the gradient in
+        # theirs, since programs keep them. The workspace is enough for any number of tokens, as the header says: no need to ask.
+        empty, at, kb = torch.empty, self._at, 16384 + 8 * pairs
+        ratio, pair_loss, margin = torch.unsafe_split_with_sizes(empty(4 * pairs, dtype=f32, device=at), (2 * pairs, pairs, pairs))
+        loss, keep = logp.new_empty(()), empty(kb, dtype=torch.uint8, device=at)
+        g = empty(n, dtype=f32, device=at) if grad else None
+        p = ratio.data_ptr()
+        self._ck(self.L.mlx_preference_loss(self.device, self._stream(), lp, rp, n, qp, pairs, beta, smoothing, scale, bool(mean), mp, wp, fp, loss.data_ptr(),
+                                            p + 8 * pairs, p + 12 * pairs, p, None if g is None else g.data_ptr(), keep.data_ptr(), kb))
+        return PreferenceResult(loss, pair_loss, margin, ratio, g)

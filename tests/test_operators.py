@@ -269,6 +269,33 @@ def test_a_tensor_written_in_place_gets_a_new_version(rc):
         assert (out._version > before[0]) == (rc != -1) and (stats._version, f._version) == before[1:]
 
 
+def test_preference_results_are_tensors_of_their_own():
+    """What comes back can be written in place, by a tensor that requires a gradient too, and kept, whatever happens to the others."""
+    ops = _on_nothing()
+    f = torch.zeros(1000)
+    r = ops.preference_loss(f, None, torch.zeros(2001, dtype=torch.int64))
+    assert r.loss.untyped_storage().nbytes() < 64 and r.loss.shape == () and r.grad.untyped_storage().nbytes() == 4000
+    w = torch.ones((), requires_grad=True)
+    kept = [(x * w).sum() for x in r]                      # (each keeps its factor for w's gradient)
+    versions = [x._version for x in r]
+    r.loss.div_(8)
+    assert [x._version - v for x, v in zip(r, versions)] == [1, 0, 0, 0, 0]
+    for k in kept[1:]:
+        k.backward()
+    for x in r:
+        x.mul_(w)
+        assert x.requires_grad
+    assert ops.preference_loss(f, None, torch.zeros(1, dtype=torch.int64)).ratio.shape == (0,)
+
+
+@pytest.mark.parametrize("pairs", [0, 1, 2, 3, 7, 8, 16, 63, 64, 100, 255, 256, 512, 1000, 100000, 2 ** 21, 2 ** 29])
+def test_preference_workspace_is_bounded_by_the_pairs(pairs):
+    L, need = operators.load_operators(), ctypes.c_size_t()
+    for each in (0, 1, 4, 5, 64, 65, 8192, 8193, 100000, 2 ** 29):
+        n = min(2 ** 31 - 2, 2 * pairs * each)
+        assert L.mlx_preference_loss_workspace(n, pairs, ctypes.byref(need)) == 0 and need.value <= 16384 + 8 * pairs
+
+
 @gpu
 def test_an_overwritten_tensor_that_a_graph_kept_is_noticed(ops):
     """A soft cap keeps its result for its backward pass; the gradient written over it must not pass for it."""
