@@ -59,8 +59,10 @@ int mlx_token_loglik_gradient(int32_t device, void *stream, int32_t type, const 
                               int32_t id_type, const void *target, const float *stats, const float *grad_logp, void *dlogits, int64_t ld_dlogits);
 
 /* Loss and gradient of n_pairs pairs of sequences, packed one behind the other: sequence s holds the tokens
- * [seq_ptr[s], seq_ptr[s+1]), s < 2 n_pairs, pair p prefers sequence p to sequence n_pairs + p. seq_ptr[2 n_pairs + 1] is ascending,
- * within [0, n_tokens] (values outside are read as the nearest bound, a sequence that ends before it begins as empty).
+ * [seq_ptr[s], seq_ptr[s+1]), s < 2 n_pairs, pair p prefers sequence p to sequence n_pairs + p. seq_ptr[2 n_pairs + 1] has to be ascending,
+ * within [0, n_tokens]. Bounds are on the device and cannot be refused: values outside are read as the nearest bound, and where they descend
+ * every access stays within the arrays, a sequence that ends before it begins counts as empty for ratio, margin and loss, and grad is unspecified
+ * (a token can then be of two sequences, or be taken for one of none).
  *   ratio[s] = sum over its tokens of logp - ref_logp   (mean != 0: divided by their number; an empty sequence has ratio 0)
  *   margin[p] = beta (ratio[p] - ratio[n_pairs + p]) + offset[p]
  *   pair_loss[p] = (1 - smoothing) log(1 + exp(-margin)) + smoothing log(1 + exp(margin))

@@ -206,8 +206,8 @@ class HipOperators:
     # -- preference -------------------------------------------------------------------------------
     def preference_loss(self, logp, ref_logp, seq_ptr, beta: float = 0.1, smoothing: float = 0.0, scale: float = 1.0, mask=None, weight=None, offset=None,
                         mean: bool = False, grad: bool = True):
-        """Loss and gradient of pairs of packed sequences: sequence s holds the tokens seq_ptr[s] .. seq_ptr[s + 1], the first half of the sequences
-        are the preferred ones. logp, ref_logp (or None) [n] float32, seq_ptr [2 pairs + 1] int64, mask (or None) [n] bool / uint8, weight, offset
+        """Loss and gradient of pairs of packed sequences: sequence s holds the tokens seq_ptr[s] .. seq_ptr[s + 1] (ascending: where they descend grad is
+        unspecified), the first half of the sequences are the preferred ones. beta, smoothing and scale are taken as 32-bit numbers. logp, ref_logp (or None) [n] float32, seq_ptr [2 pairs + 1] int64, mask (or None) [n] bool / uint8, weight, offset
         (or None) [pairs] float32. Returns loss = sum of scale * weight * pair_loss, pair_loss, margin [pairs], ratio [2 pairs] and grad [n]
         (None where grad=False)."""
         torch, f32 = self._torch, self._f32

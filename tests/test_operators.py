@@ -973,6 +973,27 @@ def test_preference_of_nothing_and_bad_bounds(ops):
 
 
 @gpu
+@pytest.mark.parametrize("n,pairs", [(40, 6), (40, 300), (3000, 7), (60000, 3)])
+def test_preference_of_descending_bounds_stays_within_its_arrays(ops, n, pairs):
+    """Bounds in any order and far outside: ratios are the sums between them, and nothing before or behind the outputs is written."""
+    g = rng(n + pairs)
+    logp = -torch.rand(n, generator=g, device="cuda")
+    seq = torch.randint(-n // 4, n + n // 4, (2 * pairs + 1,), generator=g, device="cuda")
+    seq[::5] *= 2 ** 40
+    guard, need = 64, 16384 + 8 * pairs
+    out = {k: torch.full((size + 2 * guard,), 9.0, device="cuda") for k, size in (("loss", 1), ("pair_loss", pairs), ("margin", pairs), ("ratio", 2 * pairs), ("grad", n))}
+    keep = torch.empty(need, dtype=torch.uint8, device="cuda")
+    ops._ck(ops.L.mlx_preference_loss(0, ops._stream(), logp.data_ptr(), None, n, seq.data_ptr(), pairs, 0.5, 0.0, 1.0, 0, None, None, None,
+                                      *[out[k][guard:].data_ptr() for k in ("loss", "pair_loss", "margin", "ratio", "grad")], keep.data_ptr(), need))
+    for x in out.values():
+        assert (x[:guard] == 9).all() and (x[-guard:] == 9).all()
+    bounds = [min(max(int(v), 0), n) for v in seq.cpu()]
+    sums = torch.cat([torch.zeros(1, dtype=torch.float64), logp.double().cpu().cumsum(0)])
+    want = torch.stack([sums[max(e, b)] - sums[b] for b, e in zip(bounds, bounds[1:])])
+    within(out["ratio"][guard:-guard], want, half_step(want, torch.float32) + 4 * n * 2.0 ** -53 * n)
+
+
+@gpu
 def test_preference_gradient_is_the_difference_quotient(ops):
     """Central differences of the loss in one logp, step d: off by d^2 / 6 times the third derivative (beta^3 / 8 at most, times scale) and
     by the roundings of the two losses over 2 d."""
