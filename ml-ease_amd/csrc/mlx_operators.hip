@@ -1280,7 +1280,8 @@ int check_matrix(const char *who, const char *what, const void *p, int64_t rows,
 // Matrices go past the caches' usual replacement (non-temporal) where what a call writes, or reads once and writes, is more than the memory-side
 // cache holds: the next reader would not find it there, and its write-back would run beside the next kernel. Measured, non-temporal / usual, alone
 // and with the row norms of the result taken right behind it: 8192 x 32000 bf16 loglik forward and backward 175 / 234, 299 / 348 us; 777 x 50021
-// f32 82 / 107, 120 / 123; gradient of 16384 x 4096 bf16 into 64000 rows 141 / 159, 249 / 278. Below the limit it is the other way about once there
+// f32 82 / 107, 120 / 123; gradient of 16384 x 4096 bf16 into 64000 rows 141 / 159, 249 / 278; lookup of 40000 x 4096 bf16 (328 MB) 99 / 121, 180 / 189,
+// of 10000000 x 8 f32 (320 MB) 76 / 143, 465 / 477, of 131072 x 4096 f32 (2.1 GB) 729 / 787, 1070 / 1128. Below the limit it is the other way about once there
 // is a reader: lookup of 16384 x 4096 bf16 (134 MB) 34 / 37 alone, 73 / 64 with the norms; logits of 64 MB even.
 constexpr int64_t MEMORY_SIDE_CACHE = 256ll << 20;
 bool streams(int64_t rows, int64_t width, int64_t bytes) { return rows * width > MEMORY_SIDE_CACHE / bytes; }

@@ -842,6 +842,63 @@ def test_loglik_gradient_is_the_difference_quotient(ops, classes):
         within(d[:, j], q, h * h / 36 + err / (2 * h) + 1e-6)
 
 
+# ---------------------------------------------------------------------------------------------- matrices beyond the memory-side cache
+BEYOND = 256 << 20          # bytes from which on results are written past the caches
+
+
+@gpu
+@pytest.mark.parametrize("dtype,n,width", [(torch.float32, 33000, 2048), (torch.bfloat16, 40000, 3501), (torch.float16, 33001, 4097), (torch.float32, 5000011, 14), (torch.float32, 22400001, 3),
+                                           (torch.bfloat16, 19300000, 7), (torch.float16, 16800000, 8)])
+def test_lookup_beyond_the_cache(ops, dtype, n, width):
+    assert n * width * dtype.itemsize > BEYOND
+    g = rng(width)
+    table = torch.randn(5003, width, generator=g, device="cuda").to(dtype)
+    ids = some_ids(g, n, 5003, torch.int32)
+    got, want = ops.embedding_lookup(table, ids, scale=1.7), plain_lookup(table, ids, 1.7)
+    assert torch.equal(got, want)
+    into = torch.full((n, width + 1), 9.0, device="cuda", dtype=dtype)
+    ops.embedding_lookup(table, ids, scale=1.7, out=into[:, :width])
+    assert torch.equal(into[:, :width], want) and (into[:, width] == 9).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,grad_type", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("n,width", [(1, 2049), (500, 2049), (3000, 2049), (5000, 1030), (70000, 2049), (300, 5), (9000, 3)])
+def test_gradient_beyond_the_cache(ops, dtype, grad_type, n, width):
+    """One launch, the sort in one workgroup and in many, rows with an id spared the zeros and not, one slot a row and many."""
+    rows = BEYOND // (width * grad_type.itemsize) + 1000
+    g = rng(n)
+    go = torch.randn(n, width, generator=g, device="cuda").to(dtype)
+    ids = torch.where(torch.rand(n, generator=g, device="cuda") < 0.5, torch.randint(0, rows, (n,), generator=g, device="cuda"), torch.randint(rows - 50, rows + 3, (n,), generator=g, device="cuda"))
+    got = ops.embedding_gradient(go, ids, rows, scale=1.5, dtype=grad_type)
+    start = torch.randn(rows, 1, generator=g, device="cuda").to(grad_type).expand(rows, width).contiguous()
+    out = start.clone()
+    ops.embedding_gradient(go, ids, rows, scale=1.5, out=out, accumulate=True)
+    used = torch.unique(ids[ids < rows])
+    at = torch.where(ids < rows, torch.searchsorted(used, ids), torch.full_like(ids, -1))      # (in 64 bits the rows that have an id only)
+    check_gradient(got[used], go, at, used.numel(), 1.5)
+    check_gradient(out[used], go, at, used.numel(), 1.5, before=start[used])
+    got[used] = 0
+    assert not got.any()
+    out[used] = start[used]
+    assert torch.equal(out, start)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 700), (torch.float16, 1400), (torch.bfloat16, 1400)])
+@pytest.mark.parametrize("classes", [50021, 50024])
+def test_loglik_gradient_beyond_the_cache(ops, dtype, n, classes):
+    assert 2 * n * classes * dtype.itemsize > BEYOND
+    g = rng(n + classes)
+    logits = (4 * torch.randn(n, classes, generator=g, device="cuda")).to(dtype)
+    target = some_ids(g, n, classes, torch.int64)
+    w = torch.randn(n, generator=g, device="cuda")
+    w[5] = 0
+    logp, stats = check_loglik(ops, logits, target, w)
+    want = ops.token_loglik_gradient(logits, target, stats, w)
+    assert torch.equal(ops.token_loglik_gradient(logits, target, stats, w, out=logits), want) and torch.equal(logits, want)
+
+
 # ---------------------------------------------------------------------------------------------- preference
 def exact_preference(logp, ref, seq_ptr, beta, smoothing, scale, mask, weight, offset, mean):
     """In 64 bits on the host, a loop over the sequences."""
