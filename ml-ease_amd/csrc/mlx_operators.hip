@@ -1317,9 +1317,16 @@ GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
 
 // Lanes of a row: enough that a lane has a few chunks, 8 at least; 1024 where the rows are too few to fill the chip with 256 each. The backward
 // pass cuts its rows into parts then (of BATCH chunks a lane or more, 512 workgroups in all); the forward pass does so only where a row has more
-// than LONG_ROW classes, since it needs a second launch to join the parts (64 at most: a wave's lanes): 32 rows of 128000 bf16 take 11 us of one
-// compute unit each, bound by the exponentials, and 5.8 + 3.3 us and a launch more in 16 parts.
+// than LONG_ROW classes and at least LONG_PARTS parts, since it needs a workspace and a second launch to join the parts (64 at most: a wave's lanes). One
+// launch / parts, us a call, then in a captured graph, which does not pay for the second launch's enqueuing:
+//   1 row bf16     64000: 9.5 / 13.7, 8.5 / 7.5    128000: 11.0 / 13.8, 12.2 / 7.4   160000: 12.9 / 13.6, 14.1 / 7.5    256000: 18.4 / 13.7, 20.0 / 7.7
+//   32 rows bf16   64000: 9.6 / 14.2, 9.0 / 8.0    128000: 11.5 / 13.8, 12.7 / 8.4   160000: 14.2 / 13.6, 15.3 / 9.1    256000: 19.4 / 13.7, 20.7 / 10.3
+//   32 rows f32    64000: 9.5 / 13.7, 9.7 / 8.1    128000: 13.0 / 13.8, 14.2 / 10.0  160000: 15.1 / 13.9, 17.1 / 10.6   256000: 21.4 / 13.7, 22.8 / 12.3
+//   128 rows bf16 (4 parts)                        128000: 12.1 / 14.0, 13.5 / 13.4  160000: 14.8 / 14.6, 15.8 / 15.3   256000: 20.1 / 16.7, 21.2 / 17.9
+//   256 rows bf16 (2 parts)                        128000: 14.6 / 16.9, 15.9 / 17.8  160000: 17.1 / 19.9, 18.7 / 21.1   256000: 27.5 / 29.6, 29.3 / 31.3
+// (the rule goes by the plain call: graphs of rows between 64000 and 160000 classes would gain, and plain calls lose as much).
 constexpr int64_t LONG_ROW = 160000;
+constexpr int LONG_PARTS = 4;
 struct LoglikPlan { int lanes, parts, grad_lanes, grad_parts; size_t bytes; };
 LoglikPlan loglik_plan(int64_t es, int64_t n, int64_t classes)
 {
@@ -1330,7 +1337,7 @@ LoglikPlan loglik_plan(int64_t es, int64_t n, int64_t classes)
     if (chunks > p.lanes * BATCH) p.lanes = 256;
     p.grad_lanes = p.lanes;
     p.grad_parts = n >= 512 || n == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({ 64, ceil_div(512, n), chunks / (256 * BATCH) }));
-    p.parts = classes > LONG_ROW ? p.grad_parts : 1;
+    p.parts = classes > LONG_ROW && p.grad_parts >= LONG_PARTS ? p.grad_parts : 1;
     if (n <= 512 && p.grad_parts > 1) p.lanes = 1024;
     p.bytes = p.parts > 1 ? (size_t)(n * p.parts) * sizeof(RowSum) : 0;
     return p;

@@ -842,6 +842,18 @@ def test_loglik_gradient_is_the_difference_quotient(ops, classes):
         within(d[:, j], q, h * h / 36 + err / (2 * h) + 1e-6)
 
 
+@gpu
+@pytest.mark.parametrize("dtype,n,classes", [(torch.bfloat16, 171, 160009), (torch.float32, 170, 160009), (torch.float16, 129, 160000), (torch.bfloat16, 511, 160001)])
+def test_loglik_of_long_rows(ops, dtype, n, classes):
+    """On both sides of the rule that cuts rows into parts: of 160000 classes and more, up to 170 rows and more than that."""
+    need = ctypes.c_size_t()
+    ops._ck(ops.L.mlx_token_loglik_workspace(n, classes, ctypes.byref(need)))
+    assert (need.value > 0) == (n <= 170 and classes > 160000)
+    g = rng(n)
+    logits = (4 * torch.randn(n, classes, generator=g, device="cuda")).to(dtype)
+    check_loglik(ops, logits, some_ids(g, n, classes, torch.int64))
+
+
 # ---------------------------------------------------------------------------------------------- matrices beyond the memory-side cache
 BEYOND = 256 << 20          # bytes from which on results are written past the caches
 
