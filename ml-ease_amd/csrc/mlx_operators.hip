@@ -1286,12 +1286,18 @@ int check_matrix(const char *who, const char *what, const void *p, int64_t rows,
 constexpr int64_t MEMORY_SIDE_CACHE = 256ll << 20;
 bool streams(int64_t rows, int64_t width, int64_t bytes) { return rows * width > MEMORY_SIDE_CACHE / bytes; }
 
-// Rows with an id are spared the zeros where that may be much of the table and a row is long enough to be asked about: 65536 entries of 4096 bf16 in
-// 32000 rows 221 us (frequent ids) and 211 (uniform) instead of 240 and 256, 16384 entries in 32000 rows 109 and 103 instead of 111 and 113; with a
-// quarter of the rows' number in entries 144 and 143 instead of 142 and 153, with an eighth 126 and 127 instead of 121 and 128.
-constexpr int64_t OWNER_WIDTH = 2048;
+// Rows with an id are spared the zeros where that may be much of the table and a row of grad is OWNER_BYTES or more. Without / with, us a call, uniform ids
+// into 32000 rows:
+//   entries      bf16 512        bf16 1024       f32 512         bf16 4096       f32 4096
+//   8000         33.8 / 34.9     38.9 / 39.0     38.4 / 38.2     83.1 / 79.6     152 / 138
+//   16000        35.6 / 36.9     43.1 / 41.8     42.4 / 41.0     111 / 104       195 / 167
+//   32000        39.9 / 39.8     52.5 / 49.5     50.9 / 48.4     170 / 139       268 / 220
+//   64000        47.2 / 46.7     71.9 / 67.5     72.0 / 67.3     253 / 208       389 / 318
+// with frequent ids (the k-th with a probability of about 1 / k) the difference is half of that or less, and where entries are few the marks cost more
+// than they spare: into 64000 rows of 4096 bf16 a quarter of the rows' number 142 / 144 (uniform 153 / 143), an eighth 121 / 126 (128 / 127).
+constexpr int64_t OWNER_BYTES = 2048;
 struct GradientPlan { SortPlan sort; int lpr; bool owner, few; int64_t slots, tiles, pieces; size_t key, counts, owners, part, bytes; };
-GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
+GradientPlan gradient_plan(int64_t es, int64_t gs, int64_t n_rows, int64_t width, int64_t n)       // es, gs: bytes of grad_out's and grad's elements
 {
     GradientPlan g;
     const int64_t E = 16 / es;
@@ -1308,7 +1314,7 @@ GradientPlan gradient_plan(int64_t es, int64_t n_rows, int64_t width, int64_t n)
     auto round = [](size_t b) { return (b + 255) / 256 * 256; };
     g.key = round((size_t)n * 4);
     g.counts = n <= ONE_TILE ? 0 : round((size_t)g.sort.tiles * DIGITS * 4);
-    g.owner = n > ONE_TILE && width >= OWNER_WIDTH && n >= n_rows / 2;
+    g.owner = n > ONE_TILE && width * gs >= OWNER_BYTES && n >= n_rows / 2;
     g.owners = g.owner ? round((size_t)n_rows * 4) : 0;
     g.part = g.pieces > 1 ? round((size_t)g.pieces * 2 * (size_t)g.slots * (size_t)E * 4) : 0;
     g.bytes = g.few ? 0 : 4 * g.key + g.counts + g.owners + g.part;
@@ -1410,7 +1416,7 @@ int mlx_embedding_gradient_workspace(int64_t n_rows, int64_t width, int64_t n_id
     const char *who = "mlx_embedding_gradient_workspace";
     MLX_REFUSE(!bytes, "%s: bytes is NULL", who);
     MLX_REFUSE(n_rows < 0 || n_rows > MOST || n_ids < 0 || n_ids > MOST || width < 1 || width > MOST, "%s: bad sizes", who);
-    *bytes = std::max(gradient_plan(4, n_rows, width, n_ids).bytes, gradient_plan(2, n_rows, width, n_ids).bytes);
+    *bytes = std::max({ gradient_plan(4, 4, n_rows, width, n_ids).bytes, gradient_plan(2, 2, n_rows, width, n_ids).bytes, gradient_plan(2, 4, n_rows, width, n_ids).bytes });
     return MLX_OK;
 }
 
@@ -1427,7 +1433,7 @@ int mlx_embedding_gradient(int32_t device, void *stream, int32_t type, const voi
     int rc;
     if ((rc = check_matrix(who, "grad_out", grad_out, n_ids, width, ld_grad_out, es, false)) || (rc = check_matrix(who, "grad", grad, n_rows, width, ld_grad, gs, true))) return rc;
     MLX_REFUSE(n_ids > 0 && (!ids || (uintptr_t)ids % (uintptr_t)is), "%s: ids is NULL or not aligned", who);
-    const GradientPlan plan = gradient_plan(es, n_rows, width, n_ids);
+    const GradientPlan plan = gradient_plan(es, gs, n_rows, width, n_ids);
     MLX_REFUSE(workspace_bytes < plan.bytes, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, plan.bytes);
     MLX_REFUSE(plan.bytes && (!workspace || (uintptr_t)workspace % 256), "%s: workspace is NULL or not aligned to 256 bytes", who);
     const int64_t gb = span(n_rows, width, ld_grad, gs);
