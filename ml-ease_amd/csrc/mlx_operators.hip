@@ -943,7 +943,8 @@ __global__ __launch_bounds__(64) void k_token_loglik_join(const T *__restrict__ 
     if (threadIdx.x == 0) put_loglik(logp, stats, t, all, to_float(logits[t * ld + y]));
 }
 // Backward: one read and one write of the row, bound by memory (115 to 118 us of the 174; 840 MB, some of the logits from the memory-side cache);
-// the target's class as -expm1(log p), since 1 - p would lose the digits of a p near 1.
+// the target's class as -expm1(log p), since 1 - p would lose the digits of a p near 1. log2 e and the logarithm's product with it in two parts each: with
+// one part all probabilities of a row are too large alike (5000 classes of spread 2: their sum by 9e-8 on average, 3e-9 so).
 // A workgroup takes ROWS rows of LANES lanes, or a part of a row.
 template <class T, bool NT, int LANES>
 __global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, int64_t n, int64_t classes, int64_t ld, Ids target,
@@ -955,17 +956,21 @@ __global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, 
     for (int64_t b = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; b < n * parts; b += (int64_t)gridDim.x * ROWS) {
         const int64_t t = b / parts, part = b % parts;
         const int64_t y = id_at(target, t, classes);
-        const float g = gl[t], m = stats[2 * t], log_sum = stats[2 * t + 1], ls = log_sum * LOG2E;
+        const float g = gl[t], m = stats[2 * t], log_sum = stats[2 * t + 1];
+        const float ls = log_sum * LOG2E_HI, ls_low = __builtin_fmaf(log_sum, LOG2E_HI, -ls) + log_sum * LOG2E_LO;
         const bool none = y < 0 || g == 0.0f || m == -INFINITY;
-        const T *x = logits + t * ld;
+        const T *row = logits + t * ld;
         T *o = out + t * ldo;
         const int64_t c1 = (part + 1) * step < chunks ? (part + 1) * step : chunks;
-        auto other = [&](float v) { return -(g * __builtin_amdgcn_exp2f(__builtin_fmaf(v - m, LOG2E, -ls))); };
+        auto other = [&](float v) {
+            const float x = v - m;
+            return -(g * __builtin_amdgcn_exp2f(__builtin_fmaf(x, LOG2E_HI, __builtin_fmaf(x, LOG2E_LO, -ls_low) - ls)));
+        };
         auto hit = [&](float v) { return g * -expm1f((v - m) - log_sum); };
         auto slot = [&](int64_t c, float (&f)[E]) {
             float h = 0.0f;
             const bool here = c == y / E;
-            if (here) h = hit(to_float(x[y]));
+            if (here) h = hit(to_float(row[y]));
 #pragma unroll
             for (int i = 0; i < E; i++) f[i] = other(f[i]);
             if (here)
@@ -981,18 +986,18 @@ __global__ __launch_bounds__(256) void k_token_loglik_gradient(const T *logits, 
             for (; c + (BATCH - 1) * LANES < c1; c += BATCH * LANES) {
                 float f[BATCH][E];
 #pragma unroll
-                for (int i = 0; i < BATCH; i++) load_chunk<NT>(x + (c + i * LANES) * E, f[i]);
+                for (int i = 0; i < BATCH; i++) load_chunk<NT>(row + (c + i * LANES) * E, f[i]);
 #pragma unroll
                 for (int i = 0; i < BATCH; i++) slot(c + i * LANES, f[i]);
             }
             for (; c < c1; c += LANES) {
                 float f[E];
-                load_chunk<NT>(x + c * E, f);
+                load_chunk<NT>(row + c * E, f);
                 slot(c, f);
             }
         }
         const int64_t j = chunks * E + lane;
-        if (part == parts - 1 && j < classes) o[j] = from_float<T>(none ? 0.0f : j == y ? hit(to_float(x[j])) : other(to_float(x[j])));
+        if (part == parts - 1 && j < classes) o[j] = from_float<T>(none ? 0.0f : j == y ? hit(to_float(row[j])) : other(to_float(row[j])));
     }
 }
 

@@ -812,6 +812,29 @@ def test_loglik_sums_have_no_bias(ops, dtype, n, classes):
 
 
 @gpu
+@pytest.mark.parametrize("spread", [1.0, 2.0])
+def test_loglik_gradient_has_no_bias(ops, spread):
+    """What the gradient gives to all classes but the target is -(1 - p) of it on average: the stored logarithm's rounding (half a step of 4 to 16 at most, 2.8e-7
+    rms) over 8192 rows leaves 3e-9, four times that and the mean loss of the exponentials are allowed; log2 e in one part is off by 1.33e-8 of the mean
+    logarithm of 1 / p, more than twice as much."""
+    g = rng(34)
+    n, classes = 8192, 5000
+    off, log_p = [], []
+    for a in range(0, n, 1024):
+        x = torch.randn(1024, classes, generator=g, device="cuda").mul_(spread)
+        target = torch.randint(0, classes, (1024,), generator=g, device="cuda")
+        _, stats = ops.token_loglik(x, target)
+        d = ops.token_loglik_gradient(x, target, stats, torch.ones(1024, device="cuda")).double()
+        p = x.double().softmax(1)
+        log_p.append((p * p.log()).sum(1))
+        d.scatter_(1, target[:, None], 0.0)
+        p.scatter_(1, target[:, None], 0.0)
+        off.append(-d.sum(1) / p.sum(1) - 1)
+    bound = 4 * 2.8e-7 / math.sqrt(n) + MEAN_LOSS
+    assert abs(torch.cat(off).mean()) < bound < -float(torch.cat(log_p).mean()) * ONE_PART / 2
+
+
+@gpu
 def test_margin_of_a_long_answer(ops):
     """One answer of 39000 tokens against one of 1000, from their logits, under a reference model that is near: the margin adds up the errors of 40000 log p. The
     roundings add like a random walk (4 of its deviations allowed), and what every row's sum has alike, 2e-8 at most, by the difference of the lengths."""
