@@ -1291,16 +1291,19 @@ int check_matrix(const char *who, const char *what, const void *p, int64_t rows,
 constexpr int64_t MEMORY_SIDE_CACHE = 256ll << 20;
 bool streams(int64_t rows, int64_t width, int64_t bytes) { return rows * width > MEMORY_SIDE_CACHE / bytes; }
 
-// Rows with an id are spared the zeros where that may be much of the table and a row of grad is OWNER_BYTES or more. Without / with, us a call, uniform ids
-// into 32000 rows:
-//   entries      bf16 512        bf16 1024       f32 512         bf16 4096       f32 4096
-//   8000         33.8 / 34.9     38.9 / 39.0     38.4 / 38.2     83.1 / 79.6     152 / 138
-//   16000        35.6 / 36.9     43.1 / 41.8     42.4 / 41.0     111 / 104       195 / 167
-//   32000        39.9 / 39.8     52.5 / 49.5     50.9 / 48.4     170 / 139       268 / 220
-//   64000        47.2 / 46.7     71.9 / 67.5     72.0 / 67.3     253 / 208       389 / 318
-// with frequent ids (the k-th with a probability of about 1 / k) the difference is half of that or less, and where entries are few the marks cost more
-// than they spare: into 64000 rows of 4096 bf16 a quarter of the rows' number 142 / 144 (uniform 153 / 143), an eighth 121 / 126 (128 / 127).
-constexpr int64_t OWNER_BYTES = 2048;
+// Rows with an id are spared the zeros where that may be much of the table and a row of grad is OWNER_BYTES or more. Without / with, us a call, by the bytes
+// of a row, those of the table, and entries by rows:
+//                         0.55 uniform   0.83 uniform   0.83 frequent   2 uniform    2 frequent ids (the k-th with a probability of about 1 / k)
+//   4096 (f32)   60 MB    43.1 / 41.8    47.2 / 44.6    47.7 / 46.6     66.8 / 61.4  66.6 / 63.8
+//               200 MB    87.8 / 83.1    107 / 105      109 / 109       190 / 168    191 / 181
+//               300 MB    122 / 106      146 / 125      133 / 128       231 / 207    224 / 210
+//   4096 (bf16) 200 MB    85.0 / 80.1    106 / 104      112 / 112       195 / 172    194 / 183
+//   8192 (bf16) 200 MB    84.4 / 78.4    107 / 103      108 / 105       193 / 165    188 / 172
+//   2100 (f32)  210 MB    101 / 103      124 / 129      134 / 139       164 / 156    164 / 162       (1.2 instead of 2)
+//   3000 (bf16) 180 MB                   99.8 / 102     104 / 108
+// and where entries are few the marks cost more than they spare: into 64000 rows of 4096 bf16 a quarter of the rows' number 142 / 144 (uniform 153 / 143),
+// an eighth 121 / 126 (128 / 127).
+constexpr int64_t OWNER_BYTES = 4096;
 struct GradientPlan { SortPlan sort; int lpr; bool owner, few; int64_t slots, tiles, pieces; size_t key, counts, owners, part, bytes; };
 GradientPlan gradient_plan(int64_t es, int64_t gs, int64_t n_rows, int64_t width, int64_t n)       // es, gs: bytes of grad_out's and grad's elements
 {

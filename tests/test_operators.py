@@ -500,18 +500,18 @@ def test_gradient(ops, dtype, n, rows, width):
 
 
 def test_gradient_marks_its_rows_by_their_bytes():
-    """The workspace told is enough for every pair of types: a mark a row from 2048 bytes of a float32 row on, where entries are half of the rows."""
+    """The workspace told is enough for every pair of types: a mark a row from 4096 bytes of a float32 row on, where entries are half of the rows."""
     def needs(n, rows, width):
         need = ctypes.c_size_t()
         assert operators.load_operators().mlx_embedding_gradient_workspace(rows, width, n, ctypes.byref(need)) == 0
         return need.value
-    assert needs(5000, 10000, 512) - needs(5000, 10000, 511) >= 4 * 10000
-    assert needs(5000, 10002, 512) == needs(5000, 10002, 511) and needs(4096, 100, 512) == needs(4096, 100, 511)
+    assert needs(5000, 10000, 1024) - needs(5000, 10000, 1023) >= 4 * 10000
+    assert needs(5000, 10002, 1024) == needs(5000, 10002, 1023) and needs(4096, 100, 1024) == needs(4096, 100, 1023)
 
 
 @gpu
 @pytest.mark.parametrize("dtype,grad_type", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float32)])
-@pytest.mark.parametrize("n,rows,width", [(5000, 9000, 511), (5000, 9000, 512), (5000, 10002, 512), (5000, 6000, 515), (9000, 700, 1023), (5000, 9000, 1024), (5000, 9001, 1030)])
+@pytest.mark.parametrize("n,rows,width", [(5000, 9000, 1023), (5000, 9000, 1024), (5000, 10002, 1024), (5000, 6000, 1031), (9000, 700, 2047), (5000, 9000, 2048), (5000, 9001, 2060)])
 def test_gradient_around_the_rule_of_marked_rows(ops, dtype, grad_type, n, rows, width):
     g = rng(width + rows)
     go, ids = torch.randn(n, width, generator=g, device="cuda").to(dtype), some_ids(g, n, rows, torch.int64)
