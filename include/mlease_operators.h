@@ -1,10 +1,10 @@
 /*
  * mlease_operators.h -- C-ABI of the operators on token ids, logits and pairs of answers (libmlease_hip.so).
  *
- * They stand beside the trainer's own operators (mlease_admm.h) and keep their conventions where those apply:
- *   mlx_embedding_lookup / _gradient   mlx_score_rows' lookup of coefficients by feature id, for rows of any width, and the
- *                                      column pass's gradient by sorted ids; an id the table does not hold (-1) is absent
- *   mlx_token_loglik / _gradient       mlx_test_loglik's log-likelihood, for one of many classes
+ * They stand beside the trainer's own operators (mlease_admm.h), which do not call them, and keep their conventions where those apply:
+ *   mlx_embedding_lookup / _gradient   rows of a table by id, each by itself (mlx_score_rows sums a row's coefficients), and the
+ *                                      gradient by sorted ids; an id the table does not hold (-1) is absent
+ *   mlx_token_loglik / _gradient       a log-likelihood as mlx_test_loglik's, for one of many classes
  *   mlx_preference_loss                the logistic loss and gradient with weight and offset, on the margins of pairs
  *
  * Conventions
@@ -13,6 +13,8 @@
  *   - No handle and no state: `device` is the HIP device index, `stream` a hipStream_t of that device (NULL = its null stream).
  *     A call enqueues its kernels and returns; nothing is allocated, copied to the host or waited for, so calls may be
  *     captured into a HIP graph and made from several threads at once. The calling thread's current device is left as it was.
+ *     Each launch's own status counts, not the thread's last error (hipGetLastError), which is left to whom it belongs; behind a
+ *     launch that fails nothing more is enqueued.
  *   - All data pointers are DEVICE pointers of `device` (or memory it can reach). A matrix is row-major with `ld` elements from one
  *     row to the next; outputs need ld >= the row's length, inputs may repeat rows (ld = 0). Pointers need the alignment of their
  *     element only. Outputs may not overlap inputs, except where a call says so.

@@ -15,8 +15,6 @@
 
 namespace {
 
-constexpr float LOG2E = 1.44269504088896340736f;
-
 // ---------------------------------------------------------------------------------------------- elements and 16-byte chunks
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
@@ -383,7 +381,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_one_tile(Ids ids, int n, 
 // group's entries are written at once; of the others a group leaves in LDS what it has of an id that began before it (its head, `through` where
 // that goes on behind it) and of one that begins in it and goes on (its tail). Suffix sums over the heads, doubling their reach, give every
 // tail the rest of its id; ids that cross the borders of a workgroup's entries leave a sum before (part[0]) and behind (part[1]) the border
-// for k_piece_join. The order of the additions depends on n and width only.
+// for k_piece_join. The order of the additions depends on sizes, type and ids only.
 // Bound by memory for wide rows: 16384 x 4096 bf16 38 us for 123 MB read and 75 MB written in random rows, all loads of a group on their way at
 // once; by latency for narrow ones: 195300 x 8 f32 11 us. SEG 16 leaves fewer sums to join and 40 us, 15 us here; 4 leaves 14 us of joining (7 now).
 constexpr int SEG = 8;
@@ -730,12 +728,12 @@ __global__ __launch_bounds__(256) void k_few_entries(const T *__restrict__ gout,
 // The forward pass reads through the caches as usual, so that the backward pass finds in the memory-side cache what that holds of the logits;
 // that pass reads and writes past them (8192 x 32000 bf16, both passes: 174 us so, 212 us with the forward reads non-temporal too, 204 us with
 // the writes alone, 233 us with none).
-// Forward (57 to 66 us of the 174 for 315 MB): one read of the row with the running maximum and sum of a softmax. A lane takes BATCH chunks at a
+// Forward (65 us for 315 MB, the median of traced launches, 56 at best): one read of the row with the running maximum and sum of a softmax. A lane takes BATCH chunks at a
 // time: their maximum first, one rescaling of the sum, then the exponentials. A maximum of -infinity (nothing but excluded classes so far) counts as 0 in the differences,
 // so that they stay -infinity and add 0. LANES lanes take a row; few long rows are cut into parts whose (max, sum) a second launch joins.
 // exp(t) = 2^(t log2 e) with log2 e in two parts: one part alone is off by 1.3e-8 of t in every term alike, 1e-7 of a typical row's sum, and
 // a pair's margin adds that up over hundreds of tokens (measured: margins of 512-token pairs off by 4e-6, with both parts by 5e-7).
-constexpr float LOG2E_HI = LOG2E, LOG2E_LO = 1.92596299e-8f;       // log2 e = 1.44269502162933 + 1.92596299e-8
+constexpr float LOG2E_HI = 1.44269502162933349609f, LOG2E_LO = 1.92596299e-8f;       // log2 e in two 32-bit parts
 constexpr int BATCH = 4;
 
 struct MaxSum { float m, s; };
@@ -942,7 +940,7 @@ __global__ __launch_bounds__(64) void k_token_loglik_join(const T *__restrict__ 
     for (int m = 32; m; m >>= 1) all.s += __shfl_xor(all.s, m);
     if (threadIdx.x == 0) put_loglik(logp, stats, t, all, to_float(logits[t * ld + y]));
 }
-// Backward: one read and one write of the row, bound by memory (115 to 118 us of the 174; 840 MB, some of the logits from the memory-side cache);
+// Backward: one read and one write of the row, bound by memory (120 us, the median of traced launches; 840 MB, some of the logits from the memory-side cache);
 // the target's class as -expm1(log p), since 1 - p would lose the digits of a p near 1. log2 e and the logarithm's product with it in two parts each: with
 // one part all probabilities of a row are too large alike (5000 classes of spread 2: their sum by 9e-8 on average, 3e-9 so).
 // A workgroup takes ROWS rows of LANES lanes, or a part of a row.

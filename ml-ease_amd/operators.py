@@ -1,8 +1,8 @@
 """Operators on token ids, logits and pairs of answers, as torch calls on one MI355X (C-ABI: include/mlease_operators.h).
 
-They stand beside the trainer's own: a lookup of rows by id with a scaling, and its gradient by sorted ids (what
-``HipScorer.score_rows`` and the solver's column pass do at width 1), the log-likelihood of a token among many classes with its
-gradient (``HipAdmmEngine.test_loglik_sums`` for two), and the logistic loss with weight and offset on the margins of pairs.
+They stand beside the trainer's own, which do not call them: a lookup of rows by id with a scaling (``HipScorer.score_rows`` sums a
+row's coefficients, this gives each id's row), and its gradient by sorted ids, the log-likelihood of a token among many classes with
+its gradient (``HipAdmmEngine.test_loglik_sums`` has two), and the logistic loss with weight and offset on the margins of pairs.
 
     ops = HipOperators(device=0)
     x = ops.embedding_lookup(table, ids, scale=math.sqrt(width))
